@@ -16,6 +16,9 @@ ADD, SUB, MUL, DIV, POW = range(5)
 SQRT, ERF, RELU, GELU = range(4)
 CONV_X_NHWC, CONV_Y_NHWC = 1, 2
 
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_E4M3 = range(4)
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
 MATH_MODES = {"fp32x3": MATH_FP32X3, "tf32": MATH_TF32, "fp32": MATH_FP32, "bf16": MATH_BF16}
 
 
@@ -45,6 +48,16 @@ class ConvDesc(Structure):
     _fields_ = [(n, c_int64) for n in (
         "N", "C", "H", "W", "M", "KH", "KW", "pad_h", "pad_w", "stride_h", "stride_w")] + [
         ("epilogue", c_int32), ("math_mode", c_int32)]
+
+
+class RmsnormDesc(Structure):
+    _fields_ = [(n, c_int64) for n in ("rows", "len", "x_stride", "residual_stride", "h_stride", "y_stride")] + [
+        ("type", c_int32), ("gamma_type", c_int32), ("y_type", c_int32), ("eps", c_float)]
+
+
+class QuantizeDesc(Structure):
+    _fields_ = [(n, c_int64) for n in ("rows", "len", "x_stride", "gate_stride", "q_stride")] + [
+        ("type", c_int32), ("activation", c_int32)]
 
 
 # name -> (restype, argtypes); mirrors include/b200_ops.h one to one.
@@ -80,6 +93,8 @@ SIGNATURES = {
     "b200_transpose_0213_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64]),
     "b200_maxpool2d_f32": (c_int, [c_void_p, c_void_p, c_void_p] + [c_int64] * 7),
     "b200_transpose_2d_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64]),
+    "b200_rmsnorm": (c_int, [c_void_p, POINTER(RmsnormDesc)] + [c_void_p] * 6),
+    "b200_quantize_rows": (c_int, [c_void_p, POINTER(QuantizeDesc)] + [c_void_p] * 4),
 }
 
 _lib = None

@@ -1,0 +1,401 @@
+// RMS norm with the residual's addition and 8-bit output, and the row quantiser.
+//
+//   norm      h = x + r,  y = h * rho * gamma,  rho = 1 / sqrt(mean(h^2) + eps)
+//   quantise  y = x  or  y = act(gate) * x
+//   8 bits    scale = max(max|y|, 2^-100) / 448,  code = e4m3(y / scale)
+//
+// Both are bound by memory: each input is read once, each output written once. A row stays in the registers of the
+// threads that loaded it (up to 32 values a thread). The norm needs two reductions over the row, sum(h^2) and max|y|;
+// because rho is a positive factor common to the row, max|y| = rho * max|h * gamma|, so both are taken in ONE pass
+// over the registers and joined in one exchange between warps. The maximum runs on the bit patterns of |y| as
+// unsigned integers: they order like the values, and a NaN's pattern is above infinity's, so a NaN reaches the scale.
+#include <math.h>
+
+#include "typed.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kRowsPerCta = 8;         // rows of a CTA of the warp-per-row form
+constexpr int kMaxBlock = 512;          // of a row held in registers: 32 values a thread of both inputs need ~100 registers
+constexpr int kLongBlock = 1024;
+
+struct RowParams {
+  int64_t rows;
+  int64_t x_stride, z_stride, h_stride, y_stride;  // z: residual or gate
+  const void *x, *z, *gamma;
+  void *h, *y;
+  float *scale;
+  int len;
+  float eps;
+  int activation;
+  bool gamma_f32;  // gamma is fp32 although x is not
+};
+
+// VEC adjacent values: one 16-byte access (VEC * sizeof(T) == 16), or one value.
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T *p, float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    v[0] = to_f32<T>(*p);
+  } else {
+    uint4 u;
+    // plain (not .nc): an output may be the same rows, written later by the thread that read them
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                 : "l"(p)
+                 : "memory");
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
+      else unpack2<T>(w[i], v[2 * i], v[2 * i + 1]);
+    }
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T *p, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    *p = from_f32<T>(v[0]);
+  } else if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    *reinterpret_cast<uint4 *>(p) =
+        make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void store_codes(uint8_t *p, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) *p = (uint8_t)e4m3x2(v[0], 0.f);
+  else if constexpr (VEC == 4) *reinterpret_cast<uint32_t *>(p) = e4m3x2(v[0], v[1]) | e4m3x2(v[2], v[3]) << 16;
+  else
+    *reinterpret_cast<uint2 *>(p) = make_uint2(e4m3x2(v[0], v[1]) | e4m3x2(v[2], v[3]) << 16,
+                                               e4m3x2(v[4], v[5]) | e4m3x2(v[6], v[7]) << 16);
+}
+// gamma, read by every row: cached loads
+template <typename T, int VEC>
+__device__ __forceinline__ void load_gamma(const RowParams &p, int c, float (&g)[VEC]) {
+  if (p.gamma_f32) {
+    const float *q = static_cast<const float *>(p.gamma) + c;
+    if constexpr (VEC == 1) {
+      g[0] = __ldg(q);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; i += 4) {
+        const float4 f = __ldg(reinterpret_cast<const float4 *>(q + i));
+        g[i] = f.x; g[i + 1] = f.y; g[i + 2] = f.z; g[i + 3] = f.w;
+      }
+    }
+  } else {
+    const T *q = static_cast<const T *>(p.gamma) + c;
+    if constexpr (VEC == 1) {
+      g[0] = to_f32<T>(*q);
+    } else {
+      const uint4 u = __ldg(reinterpret_cast<const uint4 *>(q));
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) g[i] = __uint_as_float(w[i]);
+        else unpack2<T>(w[i], g[2 * i], g[2 * i + 1]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ float activate(int act, float x) {
+  switch (act) {
+    case B200_ACT_RELU: return activate_t<B200_ACT_RELU>(x);
+    case B200_ACT_GELU: return activate_t<B200_ACT_GELU>(x);
+    case B200_ACT_GELU_TANH: return activate_t<B200_ACT_GELU_TANH>(x);
+    case B200_ACT_SILU: return activate_t<B200_ACT_SILU>(x);
+    default: return x;
+  }
+}
+template <int ACT, int VEC>
+__device__ __forceinline__ void gate_vec(float (&v)[VEC], const float (&z)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] *= activate_t<ACT>(z[i]);
+}
+
+__device__ __forceinline__ uint32_t warp_umax(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+
+// Sum and maximum over the threads of a row. WARP: a warp is a row. Otherwise the CTA is; `red` holds 2 x 32 words.
+template <bool WARP>
+__device__ __forceinline__ void join(float &sum, uint32_t &top, float *red) {
+  sum = warp_sum(sum);
+  top = warp_umax(top);
+  if (!WARP) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
+    if (lane == 0) {
+      red[warp] = sum;
+      red[32 + warp] = __uint_as_float(top);
+    }
+    __syncthreads();
+    // every warp joins the partial results itself, in the same order
+    sum = warp_sum(lane < nwarp ? red[lane] : 0.f);
+    top = warp_umax(lane < nwarp ? __float_as_uint(red[32 + lane]) : 0u);
+  }
+}
+
+// `top` is the pattern of max|y|: the floor keeps 448 / max finite; a NaN fails the comparison and stays.
+__device__ __forceinline__ float row_max(float top) { return top < kTinyRowMax ? kTinyRowMax : top; }
+
+// The row in registers, NV accesses of VEC values a thread. NORM: z is the residual; otherwise z is the gate.
+template <typename T, bool NORM, bool CODES, int VEC, int NV, bool WARP>
+__global__ void __launch_bounds__(WARP ? kRowsPerCta * 32 : kMaxBlock, WARP ? 2 : 1)
+rows_kernel(const RowParams p) {
+  __shared__ float red[64];
+  const int lanes = WARP ? 32 : blockDim.x;
+  const int t = WARP ? (threadIdx.x & 31) : threadIdx.x;
+  const int64_t row = WARP ? (int64_t)blockIdx.x * kRowsPerCta + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+  if (WARP && row >= p.rows) return;
+  const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
+  const T *z = static_cast<const T *>(p.z) + (p.z ? row * p.z_stride : 0);
+  float v[NV][VEC];
+  float sum = 0.f;
+  uint32_t top = 0;
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int c = (n * lanes + t) * VEC;
+    if (c < p.len) load_vec<T, VEC>(x + c, v[n]);
+  }
+  if (p.z) {
+    float w[NV][VEC];
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int c = (n * lanes + t) * VEC;
+      if (c < p.len) load_vec<T, VEC>(z + c, w[n]);
+    }
+    if (NORM) {
+      T *h = static_cast<T *>(p.h) + row * p.h_stride;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int c = (n * lanes + t) * VEC;
+        if (c < p.len) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[n][i] += w[n][i];
+          store_vec<T, VEC>(h + c, v[n]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int c = (n * lanes + t) * VEC;
+        if (c < p.len) {
+          switch (p.activation) {  // uniform
+            case B200_ACT_RELU: gate_vec<B200_ACT_RELU, VEC>(v[n], w[n]); break;
+            case B200_ACT_GELU: gate_vec<B200_ACT_GELU, VEC>(v[n], w[n]); break;
+            case B200_ACT_GELU_TANH: gate_vec<B200_ACT_GELU_TANH, VEC>(v[n], w[n]); break;
+            case B200_ACT_SILU: gate_vec<B200_ACT_SILU, VEC>(v[n], w[n]); break;
+            default: gate_vec<B200_ACT_NONE, VEC>(v[n], w[n]);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int c = (n * lanes + t) * VEC;
+    if (c < p.len) {
+      if (NORM) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum = fmaf(v[n][i], v[n][i], sum);
+        if (p.gamma) {
+          float g[VEC];
+          load_gamma<T, VEC>(p, c, g);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[n][i] *= g[i];
+        }
+      }
+      if (CODES) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(v[n][i]) & 0x7fffffffu);
+      }
+    }
+  }
+  join<WARP>(sum, top, red);
+  const float rho = NORM ? 1.f / sqrtf(sum / (float)p.len + p.eps) : 1.f;
+  float mult = rho;
+  if (CODES) {
+    const float m = row_max(__uint_as_float(top) * rho);
+    if (t == 0) p.scale[row] = m / kE4M3Max;
+    mult = rho * (kE4M3Max / m);
+  }
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int c = (n * lanes + t) * VEC;
+    if (c < p.len) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[n][i] *= mult;
+      if (CODES) store_codes<VEC>(static_cast<uint8_t *>(p.y) + row * p.y_stride + c, v[n]);
+      else store_vec<T, VEC>(static_cast<T *>(p.y) + row * p.y_stride + c, v[n]);
+    }
+  }
+}
+
+// Rows longer than the registers of a CTA: the same arithmetic, the inputs read a second time instead of kept (the
+// second read of a row of that length comes from L2). Each thread writes only where it has read, and h only in the
+// second pass, so an output may be the same rows as an input.
+template <typename T, bool NORM, bool CODES>
+__global__ void __launch_bounds__(kLongBlock)
+long_rows_kernel(const RowParams p) {
+  __shared__ float red[64];
+  const int64_t row = blockIdx.x;
+  const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
+  const T *z = static_cast<const T *>(p.z) + (p.z ? row * p.z_stride : 0);
+  T *h = static_cast<T *>(p.h) + (p.h ? row * p.h_stride : 0);
+  auto value = [&](int c) {
+    float v = to_f32<T>(x[c]);
+    if (p.z) v = NORM ? v + to_f32<T>(z[c]) : v * activate(p.activation, to_f32<T>(z[c]));
+    return v;
+  };
+  auto times_gamma = [&](float v, int c) {
+    if (!NORM || !p.gamma) return v;
+    return v * (p.gamma_f32 ? static_cast<const float *>(p.gamma)[c] : to_f32<T>(static_cast<const T *>(p.gamma)[c]));
+  };
+  float sum = 0.f;
+  uint32_t top = 0;
+  for (int c = threadIdx.x; c < p.len; c += blockDim.x) {
+    const float v = value(c);
+    if (NORM) sum = fmaf(v, v, sum);
+    if (CODES) top = max(top, __float_as_uint(times_gamma(v, c)) & 0x7fffffffu);
+  }
+  join<false>(sum, top, red);
+  const float rho = NORM ? 1.f / sqrtf(sum / (float)p.len + p.eps) : 1.f;
+  float mult = rho;
+  if (CODES) {
+    const float m = row_max(__uint_as_float(top) * rho);
+    if (threadIdx.x == 0) p.scale[row] = m / kE4M3Max;
+    mult = rho * (kE4M3Max / m);
+  }
+  for (int c = threadIdx.x; c < p.len; c += blockDim.x) {
+    const float v = value(c);
+    const float o = times_gamma(v, c) * mult;
+    if (NORM && p.z) h[c] = from_f32<T>(v);
+    if (CODES) static_cast<uint8_t *>(p.y)[row * p.y_stride + c] = (uint8_t)e4m3x2(o, 0.f);
+    else static_cast<T *>(p.y)[row * p.y_stride + c] = from_f32<T>(o);
+  }
+}
+
+template <typename T, bool NORM, bool CODES, int VEC, int NV>
+int launch_rows(cudaStream_t st, const RowParams &p, bool warp, int threads) {
+  if (warp) {
+    const int64_t ctas = (p.rows + kRowsPerCta - 1) / kRowsPerCta;
+    rows_kernel<T, NORM, CODES, VEC, NV, true><<<(unsigned)ctas, kRowsPerCta * 32, 0, st>>>(p);
+  } else {
+    rows_kernel<T, NORM, CODES, VEC, NV, false><<<(unsigned)p.rows, threads, 0, st>>>(p);
+  }
+  return check_launch("rows");
+}
+
+template <typename T, bool NORM, bool CODES>
+int dispatch(cudaStream_t st, const RowParams &p, bool vec) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const int per = vec ? V : 1;                     // values of one access
+  const int units = (p.len + per - 1) / per;       // accesses of a row (len is a multiple of V when vec)
+  // Values a thread holds at most: 32, or 16 where each needs an address and a bounds check of its own.
+  const int most = vec ? 32 : 16;
+  // A warp takes a row that fits into its registers; a longer one takes a CTA with about 16 values a thread.
+  const bool warp = units <= 32 * (most / per);
+  int nv = 1;
+  if (warp) {
+    while (nv * 32 < units) nv *= 2;
+  } else {
+    nv = 16 / per;
+    while (nv * kMaxBlock < units && nv * per < most) nv *= 2;
+    if (nv * kMaxBlock < units) {
+      long_rows_kernel<T, NORM, CODES><<<(unsigned)p.rows, kLongBlock, 0, st>>>(p);
+      return check_launch("rows(long)");
+    }
+  }
+  const int threads = ((units + nv - 1) / nv + 31) / 32 * 32;
+  if (vec) {
+    switch (nv) {
+      case 1: return launch_rows<T, NORM, CODES, V, 1>(st, p, warp, threads);
+      case 2: return launch_rows<T, NORM, CODES, V, 2>(st, p, warp, threads);
+      case 4: return launch_rows<T, NORM, CODES, V, 4>(st, p, warp, threads);
+      default: return launch_rows<T, NORM, CODES, V, 32 / V>(st, p, warp, threads);
+    }
+  }
+  if (nv <= 4) return launch_rows<T, NORM, CODES, 1, 4>(st, p, warp, threads);
+  return launch_rows<T, NORM, CODES, 1, 16>(st, p, warp, threads);
+}
+
+bool rows16(const void *p, int64_t rows, int64_t stride, int64_t elem) {
+  return aligned16(p) && (rows <= 1 || (stride * elem) % 16 == 0);
+}
+bool stride_ok(int64_t stride, int64_t len, int64_t rows, bool input) {
+  return stride >= len || rows <= 1 || (input && stride == 0);
+}
+
+int type_bytes(int type) { return type == B200_TYPE_F32 ? 4 : 2; }
+bool float_type(int type) { return type == B200_TYPE_F32 || type == B200_TYPE_F16 || type == B200_TYPE_BF16; }
+
+template <bool NORM, bool CODES>
+int by_type(cudaStream_t st, int type, const RowParams &p, bool vec) {
+  switch (type) {
+    case B200_TYPE_F32: return dispatch<float, NORM, CODES>(st, p, vec);
+    case B200_TYPE_F16: return dispatch<__half, NORM, CODES>(st, p, vec);
+    default: return dispatch<__nv_bfloat16, NORM, CODES>(st, p, vec);
+  }
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" B200_API int b200_rmsnorm(void *stream, const b200_rmsnorm_desc *desc, const void *x, const void *residual,
+                                     const void *gamma, void *h, void *y, float *scale) {
+  if (!desc) return fail(B200_EINVAL, "rmsnorm: null descriptor");
+  const b200_rmsnorm_desc &d = *desc;
+  if (d.rows < 0) return fail(B200_EINVAL, "rmsnorm: negative number of rows");
+  if (d.len < 1) return fail(B200_EINVAL, "rmsnorm: rows need at least one value");
+  if (!float_type(d.type)) return fail(B200_EINVAL, "rmsnorm: unknown type %d", d.type);
+  if (gamma && d.gamma_type != d.type && d.gamma_type != B200_TYPE_F32)
+    return fail(B200_EINVAL, "rmsnorm: gamma must have the type of x or be fp32");
+  const bool codes = d.y_type == B200_TYPE_E4M3;
+  if (!codes && d.y_type != d.type) return fail(B200_EINVAL, "rmsnorm: the output has the type of x, or is e4m3");
+  if (!(d.eps >= 0.f)) return fail(B200_EINVAL, "rmsnorm: eps must not be negative");
+  if (d.rows == 0) return B200_OK;
+  if (d.rows > 0x7fffffffLL || d.len > 0x7fffffffLL - kLongBlock)
+    return fail(B200_EUNSUPPORTED, "rmsnorm: more than 2^31 rows or values a row");
+  if (!x || !y || (codes && !scale)) return fail(B200_EINVAL, "rmsnorm: null pointer");
+  if (!residual != !h) return fail(B200_EINVAL, "rmsnorm: residual and h come together");
+  if (!stride_ok(d.x_stride, d.len, d.rows, true) || (residual && !stride_ok(d.residual_stride, d.len, d.rows, true)) ||
+      (h && !stride_ok(d.h_stride, d.len, d.rows, false)) || !stride_ok(d.y_stride, d.len, d.rows, false))
+    return fail(B200_EINVAL, "rmsnorm: a row stride is smaller than the row");
+  const int b = type_bytes(d.type);
+  const bool vec = d.len % (16 / b) == 0 && rows16(x, d.rows, d.x_stride, b) &&
+                   (!residual || (rows16(residual, d.rows, d.residual_stride, b) && rows16(h, d.rows, d.h_stride, b))) &&
+                   (!gamma || aligned16(gamma)) && rows16(y, d.rows, d.y_stride, codes ? 1 : b);
+  RowParams p = {d.rows, d.x_stride, d.residual_stride, d.h_stride, d.y_stride, x, residual, gamma, h, y, scale,
+                 (int)d.len, d.eps, B200_ACT_NONE, gamma && d.gamma_type == B200_TYPE_F32 && d.type != B200_TYPE_F32};
+  return codes ? by_type<true, true>((cudaStream_t)stream, d.type, p, vec)
+               : by_type<true, false>((cudaStream_t)stream, d.type, p, vec);
+}
+
+extern "C" B200_API int b200_quantize_rows(void *stream, const b200_quantize_desc *desc, const void *x,
+                                           const void *gate, void *q, float *scale) {
+  if (!desc) return fail(B200_EINVAL, "quantize_rows: null descriptor");
+  const b200_quantize_desc &d = *desc;
+  if (d.rows < 0) return fail(B200_EINVAL, "quantize_rows: negative number of rows");
+  if (d.len < 1) return fail(B200_EINVAL, "quantize_rows: rows need at least one value");
+  if (!float_type(d.type)) return fail(B200_EINVAL, "quantize_rows: unknown type %d", d.type);
+  if (d.activation < B200_ACT_NONE || d.activation > B200_ACT_SILU)
+    return fail(B200_EINVAL, "quantize_rows: unknown activation %d", d.activation);
+  if (!gate && d.activation != B200_ACT_NONE)
+    return fail(B200_EINVAL, "quantize_rows: an activation belongs to a gate");
+  if (d.rows == 0) return B200_OK;
+  if (d.rows > 0x7fffffffLL || d.len > 0x7fffffffLL - kLongBlock)
+    return fail(B200_EUNSUPPORTED, "quantize_rows: more than 2^31 rows or values a row");
+  if (!x || !q || !scale) return fail(B200_EINVAL, "quantize_rows: null pointer");
+  if (!stride_ok(d.x_stride, d.len, d.rows, true) || (gate && !stride_ok(d.gate_stride, d.len, d.rows, true)) ||
+      !stride_ok(d.q_stride, d.len, d.rows, false))
+    return fail(B200_EINVAL, "quantize_rows: a row stride is smaller than the row");
+  const int b = type_bytes(d.type);
+  const bool vec = d.len % (16 / b) == 0 && rows16(x, d.rows, d.x_stride, b) && (!gate || rows16(gate, d.rows, d.gate_stride, b)) &&
+                   rows16(q, d.rows, d.q_stride, 1);
+  RowParams p = {d.rows, d.x_stride, d.gate_stride, 0, d.q_stride, x, gate, nullptr, nullptr, q, scale,
+                 (int)d.len, 0.f, d.activation, false};
+  return by_type<false, true>((cudaStream_t)stream, d.type, p, vec);
+}

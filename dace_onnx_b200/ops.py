@@ -2,7 +2,8 @@
 
 Inputs are contiguous fp32 CUDA tensors (torch is used only for device memory and streams);
 every function launches on torch's current stream and returns without synchronising. There is no
-CPU path: a tensor that is not on a CUDA device is an error.
+CPU path: a tensor that is not on a CUDA device is an error. The functions of the 8-bit linear path
+(re-exported from `lowbit`) also take 16-bit and e4m3 tensors and any row stride.
 """
 import ctypes
 
@@ -11,6 +12,7 @@ import torch
 from . import _lib
 from ._lib import (ADD, DIV, EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RELU, EPI_BIAS_RESIDUAL, EPI_NONE, EPI_SCALE, ERF,
                    GELU, MATH_MODES, MUL, POW, RELU, SQRT, SUB, AttentionDesc, ConvDesc, GemmDesc, check)  # noqa: F401
+from .lowbit import empty_codes, quantize_rows, rmsnorm, rmsnorm_quantize  # noqa: F401 - typed tensors, 8-bit rows
 
 default_math_mode = "fp32x3"  # "fp32x3" | "tf32" | "bf16" | "fp32"; overridable per call
 

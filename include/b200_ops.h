@@ -253,6 +253,55 @@ B200_API int b200_transpose_2d_f32(void *stream, const float *x, float *y, int64
 B200_API int b200_maxpool2d_f32(void *stream, const float *x, float *y, int64_t planes, int64_t H, int64_t W,
                                 int64_t kh, int64_t kw, int64_t sh, int64_t sw);
 
+/* ------------------------------------------------------------------------------------------
+ * The 8-bit linear path: rows of e4m3 codes with one fp32 scale per row, the norm that produces
+ * them, and the matrix product that consumes them (16-bit operands too). No counterpart in the
+ * reference, whose nodes are fp32; the nodes they stand beside are the LayerNormalization chain
+ * and ONNXMatMul / ONNXGemm above.
+ *
+ * These entry points take typed tensors: `type` fields hold a B200_TYPE_* code. Row i of a tensor starts
+ * stride * i elements after its base, elements of a row are adjacent; any natural alignment is accepted unless an
+ * entry point says otherwise (16-byte aligned bases and rows take the 128-bit accesses). An input's row
+ * stride may be 0 (one row used for all). An output may be exactly the same rows as an input of the same type
+ * (same base and stride); overlapping otherwise is undefined.
+ * ------------------------------------------------------------------------------------------ */
+#define B200_TYPE_F32 0
+#define B200_TYPE_F16 1
+#define B200_TYPE_BF16 2
+#define B200_TYPE_E4M3 3 /* 4 exponent, 3 mantissa bits, largest value 448, no infinities */
+
+#define B200_ACT_NONE 0
+#define B200_ACT_RELU 1
+#define B200_ACT_GELU 2      /* x * 0.5 * (1 + erf(x / sqrt 2)) */
+#define B200_ACT_GELU_TANH 3 /* x * 0.5 * (1 + tanh(sqrt(2/pi) * (x + 0.044715 x^3))) */
+#define B200_ACT_SILU 4      /* x / (1 + exp(-x)) */
+
+/* Root-mean-square norm with the residual's addition: per row
+ *   h = x + residual (x without one), y = h / sqrt(mean(h^2) + eps) * gamma (1 without one), all in fp32;
+ *   h is stored rounded to `type` (only with a residual), y is stored rounded to `type` (y_type == type), or
+ *   as e4m3 (y_type == B200_TYPE_E4M3): a = max(max_j |y_j|, 2^-100), scale[row] = a / 448, code_j = y_j / scale[row]
+ *   rounded to nearest even. A NaN anywhere in a row makes its scale and its codes NaN.
+ * type: B200_TYPE_F32 / F16 / BF16; gamma_type: `type` or B200_TYPE_F32. residual and h come together or not at all;
+ * scale ([rows], adjacent) belongs to e4m3 outputs only. len >= 1. */
+typedef struct b200_rmsnorm_desc {
+  int64_t rows, len;
+  int64_t x_stride, residual_stride, h_stride, y_stride;
+  int32_t type, gamma_type, y_type;
+  float eps;
+} b200_rmsnorm_desc;
+B200_API int b200_rmsnorm(void *stream, const b200_rmsnorm_desc *desc, const void *x, const void *residual,
+                          const void *gamma, void *h, void *y, float *scale);
+
+/* Rows to e4m3 codes and scales as above, of y = x, or of y = act(gate) * x (gate not NULL; `activation` is a
+ * B200_ACT_* code and must be B200_ACT_NONE without a gate). type: B200_TYPE_F32 / F16 / BF16. */
+typedef struct b200_quantize_desc {
+  int64_t rows, len;
+  int64_t x_stride, gate_stride, q_stride;
+  int32_t type, activation;
+} b200_quantize_desc;
+B200_API int b200_quantize_rows(void *stream, const b200_quantize_desc *desc, const void *x, const void *gate, void *q,
+                                float *scale);
+
 #ifdef __cplusplus
 }
 #endif

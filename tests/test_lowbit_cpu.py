@@ -1,0 +1,63 @@
+"""Refusals of the 8-bit linear path that need no GPU: argument checks come before any CUDA call."""
+import ctypes
+
+import pytest
+import torch
+
+from dace_onnx_b200 import _lib, ops
+from dace_onnx_b200._lib import QuantizeDesc, RmsnormDesc
+from dace_onnx_b200.lowbit import _row_stride
+
+P = ctypes.c_void_p(256)  # never read: the calls below are refused
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(2, 16)
+    for call in (lambda: ops.rmsnorm(x), lambda: ops.rmsnorm_quantize(x), lambda: ops.quantize_rows(x)):
+        with pytest.raises(ValueError, match="no CPU path"):
+            call()
+    with pytest.raises(TypeError):
+        ops.rmsnorm([1.0])
+
+
+@pytest.mark.parametrize("change,args,code", [
+    (dict(rows=-1), {}, _lib.EINVAL), (dict(len=0), {}, _lib.EINVAL), (dict(type=3), {}, _lib.EINVAL),
+    (dict(gamma_type=2), {}, _lib.EINVAL), (dict(y_type=2), {}, _lib.EINVAL), (dict(eps=-1.0), {}, _lib.EINVAL),
+    (dict(eps=float("nan")), {}, _lib.EINVAL), (dict(x_stride=7), {}, _lib.EINVAL), (dict(y_stride=0), {}, _lib.EINVAL),
+    (dict(h_stride=0), {}, _lib.EINVAL), (dict(rows=1 << 31), {}, _lib.EUNSUPPORTED), (dict(len=1 << 31), {}, _lib.EUNSUPPORTED),
+    ({}, dict(x=None), _lib.EINVAL), ({}, dict(h=None), _lib.EINVAL), ({}, dict(residual=None), _lib.EINVAL),
+    ({}, dict(y=None), _lib.EINVAL), (dict(y_type=3), dict(scale=None), _lib.EINVAL), (dict(rows=0), dict(x=None), _lib.OK)])
+def test_rmsnorm_refusals(change, args, code):
+    d = RmsnormDesc(4, 8, 8, 8, 8, 8, 0, 0, 0, 1e-6)
+    for k, v in change.items():
+        setattr(d, k, v)
+    a = dict(x=P, residual=P, gamma=P, h=P, y=P, scale=P)
+    a.update(args)
+    assert _lib.load().b200_rmsnorm(None, ctypes.byref(d), a["x"], a["residual"], a["gamma"], a["h"], a["y"], a["scale"]) == code
+    assert _lib.load().b200_rmsnorm(None, None, P, P, P, P, P, P) == _lib.EINVAL
+
+
+@pytest.mark.parametrize("change,args,code", [
+    (dict(rows=-1), {}, _lib.EINVAL), (dict(len=0), {}, _lib.EINVAL), (dict(type=3), {}, _lib.EINVAL),
+    (dict(activation=5), {}, _lib.EINVAL), (dict(activation=-1), {}, _lib.EINVAL), (dict(gate_stride=7), {}, _lib.EINVAL),
+    (dict(q_stride=0), {}, _lib.EINVAL), (dict(rows=1 << 31), {}, _lib.EUNSUPPORTED), ({}, dict(x=None), _lib.EINVAL),
+    ({}, dict(gate=None), _lib.EINVAL), ({}, dict(q=None), _lib.EINVAL), ({}, dict(scale=None), _lib.EINVAL),
+    (dict(rows=0), dict(x=None), _lib.OK)])
+def test_quantize_rows_refusals(change, args, code):
+    d = QuantizeDesc(4, 8, 8, 8, 8, 0, 4)
+    for k, v in change.items():
+        setattr(d, k, v)
+    a = dict(x=P, gate=P, q=P, scale=P)
+    a.update(args)
+    assert _lib.load().b200_quantize_rows(None, ctypes.byref(d), a["x"], a["gate"], a["q"], a["scale"]) == code
+    assert _lib.load().b200_quantize_rows(None, None, P, P, P, P) == _lib.EINVAL
+
+
+def test_row_strides():
+    t = torch.zeros(4, 6, 8)
+    assert _row_stride(t) == 8 and _row_stride(t[:, :, :5]) == 8 and _row_stride(t[:, ::2]) == 16
+    assert _row_stride(t[:, :4]) is None            # the leading axes are not evenly spaced together
+    assert _row_stride(t[:1, :4]) == 8 and _row_stride(t[:, :1]) == 48
+    assert _row_stride(t.transpose(1, 2)) is None   # elements of a row apart
+    assert _row_stride(t[0, 0].expand(3, 8)) == 0
+    assert _row_stride(torch.zeros(5)) == 5 and _row_stride(torch.zeros(3, 1).t()) == 3
