@@ -60,6 +60,11 @@ class QuantizeDesc(Structure):
         ("type", c_int32), ("activation", c_int32)]
 
 
+class GemmScaledDesc(Structure):
+    _fields_ = [(n, c_int64) for n in ("M", "N", "K", "lda", "ldw", "ldy", "ldr")] + [
+        (n, c_int32) for n in ("a_scale_step", "w_scale_step", "type", "bias_type", "y_type", "activation")]
+
+
 # name -> (restype, argtypes); mirrors include/b200_ops.h one to one.
 SIGNATURES = {
     "b200_version": (c_int, []),
@@ -94,6 +99,7 @@ SIGNATURES = {
     "b200_maxpool2d_f32": (c_int, [c_void_p, c_void_p, c_void_p] + [c_int64] * 7),
     "b200_transpose_2d_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64]),
     "b200_rmsnorm": (c_int, [c_void_p, POINTER(RmsnormDesc)] + [c_void_p] * 6),
+    "b200_gemm_scaled": (c_int, [c_void_p, POINTER(GemmScaledDesc)] + [c_void_p] * 7),
     "b200_quantize_rows": (c_int, [c_void_p, POINTER(QuantizeDesc)] + [c_void_p] * 4),
 }
 

@@ -1,0 +1,802 @@
+// Matrix product on e4m3 / fp16 / bf16 operands with scales, bias, activation and residual in its epilogue:
+//   Y[m, n] = act(sa[m] * sw[n] * sum_k A[m, k] W[n, k] + bias[n]) + residual[m, n]
+//
+// Row scales are constant along K, so they leave the sum: the tensor cores multiply the codes as they are (an e4m3
+// product is exact in fp32) and the epilogue multiplies once per output.
+//
+// Two kernels, both TMA -> shared memory -> tcgen05.mma -> TMEM -> registers, warp-specialised (one loading thread, one
+// issuing thread, epilogue warps), K-blocks of 128 bytes with the 128-byte swizzle:
+//
+//   pair   many rows of A. A cluster of two CTAs computes 256 x BN outputs (rows of A are TMEM lanes), persistent, two
+//          accumulators so that the epilogue of a tile runs under the MMAs of the next.
+//   split  few rows of A, where the weights' bytes bound the product and there are fewer tiles than SMs. Operands
+//          change places: 128 rows of W are the TMEM lanes and NT rows of A the columns, so that a single token fills
+//          the tensor core's wide side with weights. K is split over the CTAs of a cluster (at most 8), whose partial
+//          sums meet in distributed shared memory in a fixed order (the same bits every time, no workspace). Lanes of
+//          a warp hold neighbouring columns of Y, so its stores are dense at any alignment: it also takes outputs
+//          whose rows the pair kernel's vector accesses cannot address.
+//
+// The tensor core adds into its fp32 accumulator with truncation, an error that grows with the number of additions. For
+// 16-bit outputs it stays far below their rounding; for fp32 outputs the sum is cut into chunks of kChunkKb K-blocks
+// whose accumulators the epilogue warps add in registers, rounding to nearest.
+//
+// Every mbarrier wait is bounded by a cycle budget, as in gemm_tcgen05.cu.
+#include <cuda.h>
+
+#include <atomic>
+#include <type_traits>
+
+#include "tc_common.cuh"
+#include "typed.cuh"
+
+namespace b200 {
+using namespace tc;
+namespace {
+
+constexpr int kRowBytes = 128;                    // bytes of K of one K-block
+constexpr int kTileBytes = 128 * kRowBytes;       // 128 rows of a K-block
+constexpr int kMmasPerKb = 4;                     // 32 bytes of K per instruction
+constexpr int kChunkKb = 4;                       // K-blocks of one in-core sum of fp32 outputs: 16 additions
+
+struct ScaledParams {
+  int64_t M, N;
+  int num_kb;
+  int num_m_tiles, num_n_tiles;
+  uint32_t idesc;
+  int a_scale_step, w_scale_step;
+  int bias_type, activation;
+  int vec;                                        // widest access to rows of Y and residual: 32 or 16 bytes (pair)
+  int64_t ldy, ldr;
+  const float *a_scale, *w_scale;
+  const void *bias, *residual;
+  void *Y;
+  unsigned *status;
+};
+
+__device__ __forceinline__ float bias_at(const ScaledParams &p, int64_t n) {
+  if (!p.bias) return 0.f;
+  switch (p.bias_type) {
+    case B200_TYPE_F32: return __ldg(static_cast<const float *>(p.bias) + n);
+    case B200_TYPE_F16: return __half2float(static_cast<const __half *>(p.bias)[n]);
+    default: return __bfloat162float(static_cast<const __nv_bfloat16 *>(p.bias)[n]);
+  }
+}
+__device__ __forceinline__ float w_scale_at(const ScaledParams &p, int64_t n) {
+  return p.w_scale ? __ldg(p.w_scale + n * p.w_scale_step) : 1.f;
+}
+__device__ __forceinline__ float a_scale_at(const ScaledParams &p, int64_t m) {
+  return p.a_scale ? __ldg(p.a_scale + m * p.a_scale_step) : 1.f;
+}
+
+// 32 bytes of a row, in one access or two
+__device__ __forceinline__ void load32(const void *p, int vec, uint32_t (&w)[8]) {
+  if (vec == 32) {
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p)
+                 : "memory");
+  } else {
+    const uint4 a = static_cast<const uint4 *>(p)[0], b = static_cast<const uint4 *>(p)[1];
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+  }
+}
+__device__ __forceinline__ void store32(void *p, int vec, const uint32_t (&w)[8]) {
+  if (vec == 32) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    static_cast<uint4 *>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    static_cast<uint4 *>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
+// Pair kernel: 32 neighbouring outputs of one row, held by one thread. sw, bs: scales and biases of these columns in
+// shared memory (broadcast reads). cols: how many of the 32 exist.
+template <typename OUT, int ACT>
+__device__ __forceinline__ void finish32_t(const ScaledParams &p, const float (&v)[32], float sa, const float *sw,
+                                           const float *bs, const OUT *r, OUT *y, int cols) {
+  constexpr int G = 32 / (int)sizeof(OUT);  // outputs of 32 bytes
+  if (cols >= 32) {
+#pragma unroll
+    for (int g = 0; g < 32; g += G) {
+      float o[G];
+#pragma unroll
+      for (int i = 0; i < G; i += 4) {
+        const float4 s = *reinterpret_cast<const float4 *>(sw + g + i), b = *reinterpret_cast<const float4 *>(bs + g + i);
+        o[i] = activate_t<ACT>(fmaf(v[g + i] * sa, s.x, b.x));
+        o[i + 1] = activate_t<ACT>(fmaf(v[g + i + 1] * sa, s.y, b.y));
+        o[i + 2] = activate_t<ACT>(fmaf(v[g + i + 2] * sa, s.z, b.z));
+        o[i + 3] = activate_t<ACT>(fmaf(v[g + i + 3] * sa, s.w, b.w));
+      }
+      uint32_t w[8];
+      if (r) {
+        load32(r + g, p.vec, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (sizeof(OUT) == 4) {
+            o[i] += __uint_as_float(w[i]);
+          } else {
+            float lo, hi;
+            unpack2<OUT>(w[i], lo, hi);
+            o[2 * i] += lo;
+            o[2 * i + 1] += hi;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (sizeof(OUT) == 4) w[i] = __float_as_uint(o[i]);
+        else w[i] = pack2<OUT>(o[2 * i], o[2 * i + 1]);
+      }
+      store32(y + g, p.vec, w);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < cols) {
+        float o = activate_t<ACT>(fmaf(v[i] * sa, sw[i], bs[i]));
+        if (r) o += to_f32<OUT>(r[i]);
+        y[i] = from_f32<OUT>(o);
+      }
+  }
+}
+template <typename OUT>
+__device__ __forceinline__ void finish32(const ScaledParams &p, const float (&v)[32], float sa, const float *sw,
+                                         const float *bs, const OUT *r, OUT *y, int cols) {
+  switch (p.activation) {  // uniform for the launch
+    case B200_ACT_RELU: finish32_t<OUT, B200_ACT_RELU>(p, v, sa, sw, bs, r, y, cols); break;
+    case B200_ACT_GELU: finish32_t<OUT, B200_ACT_GELU>(p, v, sa, sw, bs, r, y, cols); break;
+    case B200_ACT_GELU_TANH: finish32_t<OUT, B200_ACT_GELU_TANH>(p, v, sa, sw, bs, r, y, cols); break;
+    case B200_ACT_SILU: finish32_t<OUT, B200_ACT_SILU>(p, v, sa, sw, bs, r, y, cols); break;
+    default: finish32_t<OUT, B200_ACT_NONE>(p, v, sa, sw, bs, r, y, cols);
+  }
+}
+
+__device__ __forceinline__ void teardown_after_abort(int aborted) {
+  // copies may still be in flight after a wait gave up: leave them time before the shared memory goes
+  if (aborted) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) __nanosleep(1000);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// pair
+// ---------------------------------------------------------------------------------------------
+template <int BN>
+struct PairCfg {
+  static constexpr int kBHalfBytes = BN / 2 * kRowBytes;   // each CTA loads half of the tile's rows of W
+  static constexpr int kKbPerStage = 2;                    // one wait and one commit per eight MMAs
+  static constexpr int kStageBytes = kKbPerStage * (kTileBytes + kBHalfBytes);
+  static constexpr int kStages = (192 * 1024) / kStageBytes;
+  static constexpr int kTmemCols = 2 * BN;
+  static constexpr int kColsPerWarp = BN / 4;              // four warps on each quarter of the lanes
+  static constexpr int kEpilogueWarps = 16;
+  static constexpr int kThreads = 32 * (2 + kEpilogueWarps);
+  static constexpr int kStagingBytes = kEpilogueWarps * kColsPerWarp * 2 * 4;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256 + kStagingBytes;
+};
+
+// Tiles in groups of eight row tiles, column tiles across a group: the ~74 tiles in flight then share about 8 + 9 tile
+// edges of operands in L2 instead of 1 + 74.
+constexpr int kGroupM = 8;
+__device__ __forceinline__ void tile_at(const ScaledParams &p, int64_t tile, int &m_t, int &n_t) {
+  const int64_t per_group = (int64_t)kGroupM * p.num_n_tiles;
+  const int g = (int)(tile / per_group);
+  const int64_t in = tile - g * per_group;
+  const int first = g * kGroupM, rows = min(kGroupM, p.num_m_tiles - first);
+  n_t = (int)(in / rows);
+  m_t = first + (int)(in - (int64_t)n_t * rows);
+}
+
+template <bool F8, typename OUT, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::kThreads, 1)
+scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                   const ScaledParams p) {
+  using C = PairCfg<BN>;
+  constexpr bool kChunked = std::is_same<OUT, float>::value;
+  constexpr int kStages = C::kStages;
+  constexpr int kKbElems = F8 ? 128 : 64;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  float *staging = reinterpret_cast<float *>(smem + kStages * C::kStageBytes);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kStages * C::kStageBytes + C::kStagingBytes);
+  const uint32_t bar_full = smem_u32(bars);
+  const uint32_t bar_empty = bar_full + 8 * kStages;
+  const uint32_t bar_tfull = bar_empty + 8 * kStages;
+  const uint32_t bar_tempty = bar_tfull + 16;
+  __shared__ uint32_t s_tmem_base;
+  __shared__ int s_abort;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t smem_base = smem_u32(smem);
+  const uint32_t rank = cluster_ctarank();
+  const int64_t pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  const int64_t num_tiles = (int64_t)p.num_m_tiles * p.num_n_tiles;
+
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);   // even CTA: its expect_tx for the bytes of both
+      mbar_init(bar_empty + 8 * s, 1);  // each CTA: the issuer commits to both
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(bar_tfull + 8 * a, 1);                       // each CTA: the issuer commits to both
+      mbar_init(bar_tempty + 8 * a, 2 * C::kEpilogueWarps);  // even CTA: one arrival per epilogue warp of both
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(&s_tmem_base), C::kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = s_tmem_base;
+  volatile int *abort_flag = &s_abort;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      const uint32_t full_pair0 = map_to_cta(bar_full, 0);
+      for (int64_t tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+        int m_t, n_t;
+        tile_at(p, tile, m_t, n_t);
+        const int row_a = m_t * 256 + (int)rank * 128;
+        const int row_w = n_t * BN + (int)rank * (BN / 2);
+        for (int kb = 0; kb < p.num_kb; kb += C::kKbPerStage) {
+          if (!(ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 1u))) break;
+          // a K-block past the end of K is filled with zeros
+          const uint32_t stage = smem_base + s * C::kStageBytes;
+          if (rank == 0) mbar_expect_tx(bar_full + 8 * s, 2 * C::kStageBytes);
+#pragma unroll
+          for (int h = 0; h < C::kKbPerStage; ++h) {
+            const uint32_t a_dst = stage + h * kTileBytes;
+            const uint32_t w_dst = stage + C::kKbPerStage * kTileBytes + h * C::kBHalfBytes;
+            const int k0 = (kb + h) * kKbElems;
+            if (rank == 0) {
+              tma_load_2d(a_dst, &map_a, bar_full + 8 * s, k0, row_a);
+              tma_load_2d(w_dst, &map_w, bar_full + 8 * s, k0, row_w);
+            } else {
+              tma_load_2d_pair(a_dst, &map_a, full_pair0 + 8 * s, k0, row_a);
+              tma_load_2d_pair(w_dst, &map_w, full_pair0 + 8 * s, k0, row_w);
+            }
+          }
+          if (++s == kStages) { s = 0; ph ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t kStage16 = C::kStageBytes >> 4;
+      const uint64_t a_desc0 = make_smem_desc(smem_base, 16, 1024, kLayoutSw128);
+      const uint64_t w_desc0 = make_smem_desc(smem_base + C::kKbPerStage * kTileBytes, 16, 1024, kLayoutSw128);
+      const uint32_t idesc = p.idesc;
+      const int chunk = kChunked ? kChunkKb : p.num_kb + C::kKbPerStage;  // a multiple of the stage, or everything
+      int s = 0, acc = 0;
+      uint32_t ph = 0, acc_ph = 0;
+      bool ok = true;
+      for (int64_t tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+        for (int kb0 = 0; kb0 < p.num_kb && ok; kb0 += chunk) {
+          if (!(ok = mbar_wait(bar_tempty + 8 * acc, acc_ph ^ 1, abort_flag, p.status, 2u))) break;
+          tc_fence_after();
+          const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+          const int kb_end = min(kb0 + chunk, p.num_kb);
+          for (int kb = kb0; kb < kb_end; kb += C::kKbPerStage) {
+            if (!(ok = mbar_wait(bar_full + 8 * s, ph, abort_flag, p.status, 4u))) break;
+            tc_fence_after();
+            const uint64_t a_d = a_desc0 + (uint32_t)s * kStage16, w_d = w_desc0 + (uint32_t)s * kStage16;
+#pragma unroll
+            for (int h = 0; h < C::kKbPerStage; ++h)
+#pragma unroll
+              for (int k = 0; k < kMmasPerKb; ++k) {
+                const uint64_t a = a_d + h * (kTileBytes >> 4) + 2 * k, w = w_d + h * (C::kBHalfBytes >> 4) + 2 * k;
+                const uint32_t accumulate = (h > 0 || k > 0 || kb > kb0) ? 1u : 0u;
+                if (F8) umma_f8_pair(d_tmem, a, w, idesc, accumulate);
+                else umma_bf16_pair(d_tmem, a, w, idesc, accumulate);
+              }
+            umma_commit_pair_both(bar_empty + 8 * s, 3);
+            if (++s == kStages) { s = 0; ph ^= 1; }
+          }
+          if (!ok) break;
+          umma_commit_pair_both(bar_tfull + 8 * acc, 3);
+          if (++acc == 2) { acc = 0; acc_ph ^= 1; }
+        }
+      }
+    }
+  } else {
+    const int ew = warp - 2, quarter = warp & 3;
+    const int col0 = (ew >> 2) * C::kColsPerWarp;
+    float *sw = staging + ew * (2 * C::kColsPerWarp), *bs = sw + C::kColsPerWarp;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + col0;
+    const int chunks = kChunked ? (p.num_kb + kChunkKb - 1) / kChunkKb : 1;
+    int acc = 0;
+    uint32_t acc_ph = 0;
+    bool ok = true;
+    for (int64_t tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+      int m_t, n_t;
+      tile_at(p, tile, m_t, n_t);
+      const int64_t m = (int64_t)m_t * 256 + (int)rank * 128 + quarter * 32 + lane;
+      const int64_t n0 = (int64_t)n_t * BN + col0;
+      // this warp's columns: scales and biases to shared memory, while the MMAs run
+      __syncwarp();
+      for (int c = lane; c < C::kColsPerWarp; c += 32) {
+        const bool in = n0 + c < p.N;
+        sw[c] = in ? w_scale_at(p, n0 + c) : 0.f;
+        bs[c] = in ? bias_at(p, n0 + c) : 0.f;
+      }
+      __syncwarp();
+      const bool row_in = m < p.M;
+      const float sa = row_in ? a_scale_at(p, m) : 0.f;
+      OUT *y = static_cast<OUT *>(p.Y) + m * p.ldy + n0;
+      const OUT *r = p.residual ? static_cast<const OUT *>(p.residual) + m * p.ldr + n0 : nullptr;
+      auto emit = [&](const float (&v)[32], int c) {
+        const int64_t left = p.N - n0 - c;
+        if (row_in && left > 0) finish32<OUT>(p, v, sa, sw + c, bs + c, r ? r + c : nullptr, y + c, left < 32 ? (int)left : 32);
+      };
+      if (kChunked) {
+        float sum[C::kColsPerWarp / 32][32] = {};
+        for (int ch = 0; ch < chunks; ++ch) {
+          if (!(ok = mbar_wait(bar_tfull + 8 * acc, acc_ph, abort_flag, p.status, 8u))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < C::kColsPerWarp; c += 16) {
+            uint32_t t[16];
+            tmem_ld16(lane_addr + (uint32_t)(acc * BN + c), t);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sum[c / 32][c % 32 + j] += __uint_as_float(t[j]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(bar_tempty + 8 * acc, 0));
+          if (++acc == 2) { acc = 0; acc_ph ^= 1; }
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < C::kColsPerWarp / 32; ++c) emit(sum[c], 32 * c);
+      } else {
+        if (!(ok = mbar_wait(bar_tfull + 8 * acc, acc_ph, abort_flag, p.status, 8u))) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < C::kColsPerWarp; c += 32) {
+          uint32_t t[32];
+          float v[32];
+          __syncwarp();
+          tmem_ld32(lane_addr + (uint32_t)(acc * BN + c), t);
+          tmem_ld_wait();
+          if (c + 32 >= C::kColsPerWarp) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(bar_tempty + 8 * acc, 0));
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(t[j]);
+          emit(v, c);
+        }
+        if (++acc == 2) { acc = 0; acc_ph ^= 1; }
+      }
+    }
+  }
+
+  // neither CTA may leave while its partner can still signal its barriers or read its shared memory
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  teardown_after_abort(s_abort);
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, C::kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// split
+// ---------------------------------------------------------------------------------------------
+template <int NT, bool CHUNKED>
+struct SplitCfg {
+  static constexpr int kStageBytes = kTileBytes + NT * kRowBytes;
+  // two CTAs on an SM (one for NT = 256), so that one's start and end run under the other's loads
+  static constexpr int kStages = NT == 256 ? 4 : NT == 128 ? 3 : NT == 64 ? 4 : NT == 32 ? 5 : 6;
+  static constexpr int kCtasPerSm = NT == 256 ? 1 : 2;
+  static constexpr int kWarpsPerQuarter = NT <= 64 ? 1 : NT / 64;
+  static constexpr int kColsPerWarp = NT / kWarpsPerQuarter;   // at most 64 sums in a thread's registers
+  static constexpr int kEpilogueWarps = 4 * kWarpsPerQuarter;
+  static constexpr int kThreads = 32 * (2 + kEpilogueWarps);
+  static constexpr int kAccCols = NT < 32 ? 32 : NT;
+  static constexpr int kTmemCols = CHUNKED ? 2 * kAccCols : kAccCols;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
+  static_assert(NT * 128 * 4 <= kStages * kStageBytes, "partial sums take the place of the stages");
+};
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Outputs of this CTA: its share of the tile's rows of A (rank, rank + S, ...), for W row n of this thread.
+template <typename OUT, int ACT>
+__device__ __forceinline__ void finish_split_t(const ScaledParams &p, uint32_t partial, int ranks, int rank, int first,
+                                               int step, int64_t m0, int rows, int64_t n) {
+  const float sw = w_scale_at(p, n), bias = bias_at(p, n);
+  uint32_t base[8];
+#pragma unroll
+  for (int s = 0; s < 8; ++s) base[s] = s < ranks ? map_to_cta(partial, s) : 0u;
+  OUT *y = static_cast<OUT *>(p.Y) + m0 * p.ldy + n;
+  const OUT *r = p.residual ? static_cast<const OUT *>(p.residual) + m0 * p.ldr + n : nullptr;
+#pragma unroll 4
+  for (int t = rank + first * ranks; t < rows; t += step * ranks) {
+    float v = 0.f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      if (s < ranks) v += ld_cluster(base[s] + (uint32_t)t * 512);
+    float o = activate_t<ACT>(fmaf(v * a_scale_at(p, m0 + t), sw, bias));
+    if (r) o += to_f32<OUT>(r[t * p.ldr]);
+    y[t * p.ldy] = from_f32<OUT>(o);
+  }
+}
+
+template <bool F8, typename OUT, int NT>
+__global__ void __launch_bounds__(SplitCfg<NT, std::is_same<OUT, float>::value>::kThreads,
+                                  SplitCfg<NT, std::is_same<OUT, float>::value>::kCtasPerSm)
+scaled_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                    const ScaledParams p, const int ranks) {
+  constexpr bool kChunked = std::is_same<OUT, float>::value;
+  using C = SplitCfg<NT, kChunked>;
+  constexpr int kStages = C::kStages;
+  constexpr int kKbElems = F8 ? 128 : 64;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kStages * C::kStageBytes);
+  const uint32_t bar_full = smem_u32(bars);
+  const uint32_t bar_empty = bar_full + 8 * kStages;
+  const uint32_t bar_tfull = bar_empty + 8 * kStages;
+  const uint32_t bar_tempty = bar_tfull + 16;
+  __shared__ uint32_t s_tmem_base;
+  __shared__ int s_abort;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t smem_base = smem_u32(smem);
+  const int rank = (int)cluster_ctarank();
+  const int64_t tile = blockIdx.x / ranks;
+  const int n_t = (int)(tile / p.num_m_tiles), m_t = (int)(tile - (int64_t)n_t * p.num_m_tiles);
+  const int kb_begin = (int)((int64_t)p.num_kb * rank / ranks), kb_end = (int)((int64_t)p.num_kb * (rank + 1) / ranks);
+
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(bar_tfull + 8 * a, 1);
+      mbar_init(bar_tempty + 8 * a, C::kEpilogueWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&s_tmem_base), C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = s_tmem_base;
+  volatile int *abort_flag = &s_abort;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 1u)) break;
+        const uint32_t stage = smem_base + s * C::kStageBytes;
+        mbar_expect_tx(bar_full + 8 * s, C::kStageBytes);
+        tma_load_2d(stage, &map_w, bar_full + 8 * s, kb * kKbElems, n_t * 128);
+        tma_load_2d(stage + kTileBytes, &map_a, bar_full + 8 * s, kb * kKbElems, m_t * NT);
+        if (++s == kStages) { s = 0; ph ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint64_t w_desc0 = make_smem_desc(smem_base, 16, 1024, kLayoutSw128);
+      const uint64_t a_desc0 = make_smem_desc(smem_base + kTileBytes, 16, 1024, kLayoutSw128);
+      const int chunk = kChunked ? kChunkKb : p.num_kb;
+      int s = 0, acc = 0;
+      uint32_t ph = 0, acc_ph = 0;
+      bool ok = true;
+      for (int kb0 = kb_begin; kb0 < kb_end && ok; kb0 += chunk) {
+        if (!(ok = mbar_wait(bar_tempty + 8 * acc, acc_ph ^ 1, abort_flag, p.status, 2u))) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * C::kAccCols);
+        for (int kb = kb0; kb < min(kb0 + chunk, kb_end); ++kb) {
+          if (!(ok = mbar_wait(bar_full + 8 * s, ph, abort_flag, p.status, 4u))) break;
+          tc_fence_after();
+          const uint64_t w_d = w_desc0 + (uint32_t)s * (C::kStageBytes >> 4);
+          const uint64_t a_d = a_desc0 + (uint32_t)s * (C::kStageBytes >> 4);
+#pragma unroll
+          for (int k = 0; k < kMmasPerKb; ++k) {
+            const uint32_t accumulate = (k > 0 || kb > kb0) ? 1u : 0u;
+            if (F8) umma_f8(d_tmem, w_d + 2 * k, a_d + 2 * k, p.idesc, accumulate);
+            else umma_bf16(d_tmem, w_d + 2 * k, a_d + 2 * k, p.idesc, accumulate);
+          }
+          umma_commit(bar_empty + 8 * s);
+          if (++s == kStages) { s = 0; ph ^= 1; }
+        }
+        if (!ok) break;
+        umma_commit(bar_tfull + 8 * acc);
+        if (kChunked && ++acc == 2) { acc = 0; acc_ph ^= 1; }
+      }
+    }
+  } else {
+    const int ew = warp - 2, quarter = warp & 3;
+    const int col0 = (ew >> 2) * C::kColsPerWarp;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + col0;
+    const int chunks = kChunked ? (kb_end - kb_begin + kChunkKb - 1) / kChunkKb : 1;
+    float sum[C::kColsPerWarp] = {};
+    int acc = 0;
+    uint32_t acc_ph = 0;
+    bool ok = true;
+    for (int ch = 0; ch < chunks; ++ch) {
+      if (!(ok = mbar_wait(bar_tfull + 8 * acc, acc_ph, abort_flag, p.status, 8u))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < C::kColsPerWarp; c += 16) {
+        uint32_t t[16];
+        tmem_ld16(lane_addr + (uint32_t)(acc * C::kAccCols + c), t);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum[c + j] += __uint_as_float(t[j]);
+      }
+      if (kChunked) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_tempty + 8 * acc);
+        if (++acc == 2) { acc = 0; acc_ph ^= 1; }
+      }
+    }
+    if (ok) {
+      // the last accumulator is complete, so every load has landed and every MMA has read its stage: the
+      // stages' memory now takes the partial sums, [row of A][row of W]
+      float *partial = reinterpret_cast<float *>(smem) + quarter * 32 + lane;
+#pragma unroll
+      for (int j = 0; j < C::kColsPerWarp; ++j) partial[(col0 + j) * 128] = sum[j];
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();  // every CTA's partial sums are in place
+  if (warp >= 2) {
+    const int64_t n = (int64_t)n_t * 128 + (warp & 3) * 32 + lane;
+    const int64_t m0 = (int64_t)m_t * NT;
+    const int rows = (int)min((int64_t)NT, p.M - m0);
+    const uint32_t partial = smem_base + ((warp & 3) * 32 + lane) * 4;
+    const int first = (warp - 2) >> 2;
+    constexpr int step = C::kWarpsPerQuarter;
+    if (n < p.N) {
+      switch (p.activation) {
+        case B200_ACT_RELU: finish_split_t<OUT, B200_ACT_RELU>(p, partial, ranks, rank, first, step, m0, rows, n); break;
+        case B200_ACT_GELU: finish_split_t<OUT, B200_ACT_GELU>(p, partial, ranks, rank, first, step, m0, rows, n); break;
+        case B200_ACT_GELU_TANH:
+          finish_split_t<OUT, B200_ACT_GELU_TANH>(p, partial, ranks, rank, first, step, m0, rows, n);
+          break;
+        case B200_ACT_SILU: finish_split_t<OUT, B200_ACT_SILU>(p, partial, ranks, rank, first, step, m0, rows, n); break;
+        default: finish_split_t<OUT, B200_ACT_NONE>(p, partial, ranks, rank, first, step, m0, rows, n);
+      }
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();  // no CTA leaves while another reads its partial sums
+  teardown_after_abort(s_abort);
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C::kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------
+template <typename Kernel>
+int raise_smem(Kernel kern, int bytes, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(B200_ECUDA, "gemm_scaled: bad device");
+  if (done.load(std::memory_order_relaxed) >> dev & 1) return B200_OK;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return fail(B200_ECUDA, "gemm_scaled: cannot set dynamic shared memory to %d", bytes);
+  done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return B200_OK;
+}
+
+struct Plan {
+  bool pair;
+  int cols;   // pair: BN; split: NT
+  int ranks;  // split: CTAs over which K is split
+};
+
+struct Operands {
+  const void *A, *W;
+  int64_t K, a_pitch, w_pitch;
+  int type;
+};
+
+template <bool F8, typename OUT, int BN>
+int launch_pair(cudaStream_t st, const Operands &o, ScaledParams &p) {
+  using C = PairCfg<BN>;
+  auto kern = scaled_pair_kernel<F8, OUT, BN>;
+  static std::atomic<uint64_t> smem_set{0};
+  if (int rc = raise_smem(kern, C::kSmemBytes, smem_set)) return rc;
+  // the clusters the device holds at once: a persistent grid must not exceed them (per device, never changes)
+  static std::atomic<int> max_pairs[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(B200_ECUDA, "gemm_scaled: bad device");
+  if (max_pairs[dev].load(std::memory_order_relaxed) == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kNumSMs, 1, 1);
+    cfg.blockDim = dim3(C::kThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1)
+      return fail(B200_ECUDA, "gemm_scaled: cudaOccupancyMaxActiveClusters failed");
+    max_pairs[dev].store(n, std::memory_order_relaxed);
+  }
+  CUtensorMap ma, mw;
+  if (int rc = encode_map_rows(&ma, o.A, o.type, o.K, p.M, o.a_pitch, 128)) return rc;
+  if (int rc = encode_map_rows(&mw, o.W, o.type, o.K, p.N, o.w_pitch, BN / 2)) return rc;
+  p.num_m_tiles = (int)((p.M + 255) / 256);
+  p.num_n_tiles = (int)((p.N + BN - 1) / BN);
+  p.idesc |= (uint32_t)(BN >> 3) << 17 | (uint32_t)(256 >> 4) << 24;
+  const int64_t tiles = (int64_t)p.num_m_tiles * p.num_n_tiles, cap = max_pairs[dev].load(std::memory_order_relaxed);
+  kern<<<(unsigned)(2 * (tiles < cap ? tiles : cap)), C::kThreads, C::kSmemBytes, st>>>(ma, mw, p);
+  return check_launch("gemm_scaled(pair)");
+}
+
+template <bool F8, typename OUT, int NT>
+int launch_split(cudaStream_t st, const Operands &o, ScaledParams &p, int ranks) {
+  using C = SplitCfg<NT, std::is_same<OUT, float>::value>;
+  auto kern = scaled_split_kernel<F8, OUT, NT>;
+  static std::atomic<uint64_t> smem_set{0};
+  if (int rc = raise_smem(kern, C::kSmemBytes, smem_set)) return rc;
+  CUtensorMap ma, mw;
+  if (int rc = encode_map_rows(&ma, o.A, o.type, o.K, p.M, o.a_pitch, NT)) return rc;
+  if (int rc = encode_map_rows(&mw, o.W, o.type, o.K, p.N, o.w_pitch, 128)) return rc;
+  p.num_m_tiles = (int)((p.M + NT - 1) / NT);
+  p.num_n_tiles = (int)((p.N + 127) / 128);
+  p.idesc |= (uint32_t)(NT >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+  const int64_t ctas = (int64_t)p.num_m_tiles * p.num_n_tiles * ranks;
+  if (ctas > 0x7fffffffLL) return fail(B200_EUNSUPPORTED, "gemm_scaled: too many tiles");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+  cfg.blockDim = dim3(C::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)ranks;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kern, ma, mw, p, ranks);
+  return check_launch("gemm_scaled(split)");
+}
+
+template <bool F8, typename OUT>
+int launch_plan(cudaStream_t st, const Operands &o, ScaledParams &p, const Plan &plan) {
+  if (plan.pair) return plan.cols == 256 ? launch_pair<F8, OUT, 256>(st, o, p) : launch_pair<F8, OUT, 128>(st, o, p);
+  switch (plan.cols) {
+    case 16: return launch_split<F8, OUT, 16>(st, o, p, plan.ranks);
+    case 32: return launch_split<F8, OUT, 32>(st, o, p, plan.ranks);
+    case 64: return launch_split<F8, OUT, 64>(st, o, p, plan.ranks);
+    case 128: return launch_split<F8, OUT, 128>(st, o, p, plan.ranks);
+    default: return launch_split<F8, OUT, 256>(st, o, p, plan.ranks);
+  }
+}
+
+int type_bytes(int type) { return type == B200_TYPE_F32 ? 4 : type == B200_TYPE_E4M3 ? 1 : 2; }
+
+Plan choose(const b200_gemm_scaled_desc &d, bool vector_rows) {
+  const int64_t kb = (d.K * type_bytes(d.type) + kRowBytes - 1) / kRowBytes;
+  if (vector_rows && d.M > 256) return Plan{true, d.N > 128 ? 256 : 128, 1};
+  const int nt = d.M <= 16 ? 16 : d.M <= 32 ? 32 : d.M <= 64 ? 64 : d.M <= 128 ? 128 : 256;
+  const int64_t tiles = (d.N + 127) / 128 * ((d.M + nt - 1) / nt);
+  int ranks = 1;
+  while (ranks < 8 && tiles * ranks * 2 <= kNumSMs * (nt == 256 ? 1 : 2) && kb >= 4 * ranks) ranks *= 2;
+  return Plan{false, nt, ranks};
+}
+
+int run_plan(cudaStream_t st, const b200_gemm_scaled_desc &d, const Plan &plan, int vec, const void *A, const void *W,
+             const float *a_scale, const float *w_scale, const void *bias, const void *residual, void *Y) {
+  const int b = type_bytes(d.type);
+  ScaledParams p = {};
+  p.M = d.M;
+  p.N = d.N;
+  p.num_kb = (int)((d.K * b + kRowBytes - 1) / kRowBytes);
+  p.idesc = d.type == B200_TYPE_BF16 ? make_idesc_bf16(0, 0) : make_idesc_fp16_or_e4m3(0, 0);
+  p.a_scale_step = d.a_scale_step;
+  p.w_scale_step = d.w_scale_step;
+  p.bias_type = d.bias_type;
+  p.activation = d.activation;
+  p.vec = vec;
+  p.ldy = d.ldy;
+  p.ldr = d.ldr;
+  p.a_scale = a_scale;
+  p.w_scale = w_scale;
+  p.bias = bias;
+  p.residual = residual;
+  p.Y = Y;
+  p.status = device_status_ptr();
+  if (!p.status) return fail(B200_ECUDA, "gemm_scaled: device status word unavailable");
+  const Operands o = {A, W, d.K, d.lda * b, d.ldw * b, d.type};
+  const bool f8 = d.type == B200_TYPE_E4M3;
+  switch (d.y_type) {
+    case B200_TYPE_F32: return f8 ? launch_plan<true, float>(st, o, p, plan) : launch_plan<false, float>(st, o, p, plan);
+    case B200_TYPE_F16: return f8 ? launch_plan<true, __half>(st, o, p, plan) : launch_plan<false, __half>(st, o, p, plan);
+    default:
+      return f8 ? launch_plan<true, __nv_bfloat16>(st, o, p, plan) : launch_plan<false, __nv_bfloat16>(st, o, p, plan);
+  }
+}
+
+// Widest access with which every row of `q` can be read or written: 32, 16 or fewer (0) bytes.
+int row_access(const void *q, int64_t rows, int64_t ld, int bytes) {
+  const uint64_t bits = reinterpret_cast<uintptr_t>(q) | (rows > 1 ? (uint64_t)(ld * bytes) : 0);
+  return bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : 0;
+}
+
+bool is_float(int type) { return type == B200_TYPE_F32 || type == B200_TYPE_F16 || type == B200_TYPE_BF16; }
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" B200_API int b200_gemm_scaled(void *stream, const b200_gemm_scaled_desc *desc, const void *A, const void *W,
+                                         const float *a_scale, const float *w_scale, const void *bias,
+                                         const void *residual, void *Y) {
+  if (!desc) return fail(B200_EINVAL, "gemm_scaled: null descriptor");
+  const b200_gemm_scaled_desc &d = *desc;
+  if (d.M < 0 || d.N < 0) return fail(B200_EINVAL, "gemm_scaled: negative extent");
+  if (d.K < 1) return fail(B200_EINVAL, "gemm_scaled: K must be at least 1");
+  if (d.type != B200_TYPE_E4M3 && d.type != B200_TYPE_F16 && d.type != B200_TYPE_BF16)
+    return fail(B200_EINVAL, "gemm_scaled: operands are e4m3, fp16 or bf16, not type %d", d.type);
+  if (!is_float(d.y_type)) return fail(B200_EINVAL, "gemm_scaled: unknown output type %d", d.y_type);
+  if (bias && !is_float(d.bias_type)) return fail(B200_EINVAL, "gemm_scaled: unknown bias type %d", d.bias_type);
+  if (d.activation < B200_ACT_NONE || d.activation > B200_ACT_SILU)
+    return fail(B200_EINVAL, "gemm_scaled: unknown activation %d", d.activation);
+  if ((a_scale && (d.a_scale_step < 0 || d.a_scale_step > 1)) || (w_scale && (d.w_scale_step < 0 || d.w_scale_step > 1)))
+    return fail(B200_EINVAL, "gemm_scaled: scale steps are 0 or 1");
+  if (d.M == 0 || d.N == 0) return B200_OK;
+  if (!A || !W || !Y) return fail(B200_EINVAL, "gemm_scaled: null pointer");
+  if ((d.lda < d.K && d.M > 1) || (d.ldw < d.K && d.N > 1) || (d.ldy < d.N && d.M > 1) ||
+      (residual && d.ldr < d.N && d.M > 1))
+    return fail(B200_EINVAL, "gemm_scaled: leading dimension smaller than the row length");
+  if (d.M > 0x7fffff00LL || d.N > 0x7fffff00LL || d.K > 0x7fffff00LL)
+    return fail(B200_EUNSUPPORTED, "gemm_scaled: an extent is too large");
+  const int b = type_bytes(d.type), yb = type_bytes(d.y_type);
+  b200_gemm_scaled_desc e = d;
+  // one row: its stride is never used, any valid one will do for the tensor map
+  const int64_t pitch = (d.K * b + 15) / 16 * 16 / b;
+  if (e.M == 1) e.lda = pitch;
+  if (e.N == 1) e.ldw = pitch;
+  if (!aligned16(A) || !aligned16(W) || e.lda * b % 16 || e.ldw * b % 16)
+    return fail(B200_EUNSUPPORTED, "gemm_scaled: A and W need 16-byte aligned bases and row strides of multiples of 16 bytes");
+  if (e.lda * b >= (1LL << 40) || e.ldw * b >= (1LL << 40)) return fail(B200_EUNSUPPORTED, "gemm_scaled: a row stride is too large");
+  int vec = row_access(Y, e.M, e.ldy, yb);
+  if (residual) vec = min(vec, row_access(residual, e.M, e.ldr, yb));
+  return run_plan((cudaStream_t)stream, e, choose(e, vec >= 16), vec, A, W, a_scale, w_scale, bias, residual, Y);
+}

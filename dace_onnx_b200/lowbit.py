@@ -11,10 +11,11 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import ACTIVATIONS, TYPE_BF16, TYPE_E4M3, TYPE_F16, TYPE_F32, QuantizeDesc, RmsnormDesc, check
+from ._lib import ACTIVATIONS, TYPE_BF16, TYPE_E4M3, TYPE_F16, TYPE_F32, GemmScaledDesc, QuantizeDesc, RmsnormDesc, check
 
 FLOAT_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
 E4M3 = torch.float8_e4m3fn
+OPERAND_TYPES = {E4M3: TYPE_E4M3, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
 
 
 def _act(activation):
@@ -201,3 +202,140 @@ def quantize_rows(x, *, gate=None, activation=None, out=None, scale=None):
     _call(_lib.load().b200_quantize_rows, x.get_device(), ctypes.byref(d), xr.data_ptr(),
           None if gr is None else gr.data_ptr(), out.data_ptr(), scale.data_ptr())
     return out, scale
+
+
+def _operand(t, name, code, like):
+    """(tensor, row stride) as the product reads it: 16-byte aligned rows; a copy in that layout for any other."""
+    s = _row_stride(t)
+    size = 1 if code == TYPE_E4M3 else 2
+    if s is None or t.data_ptr() % 16 or ((s * size) % 16 and t.numel() > t.shape[-1]) or (s == 0 and t.numel() > t.shape[-1]):
+        k = t.shape[-1]
+        pitch = -(-k * size // 16) * 16 // size
+        padded = torch.empty(t.shape[:-1] + (pitch,), device=t.device, dtype=t.dtype)[..., :k]
+        padded.copy_(t)
+        return padded, pitch
+    return t, s
+
+
+def _scale_operand(t, name, rows, like):
+    """(tensor, step) of a scale operand: one entry, or one a row."""
+    if t is None:
+        return None, 0
+    _tensor(t, name, like)
+    if t.dtype != torch.float32:
+        raise TypeError("%s must be float32, got %s" % (name, t.dtype))
+    if t.numel() == 1:
+        return t, 0
+    if t.numel() != rows:
+        raise ValueError("%s must have one entry, or one for each of the %d rows" % (name, rows))
+    return t.contiguous(), 1
+
+
+def matmul_scaled(A, W, *, a_scale=None, w_scale=None, bias=None, activation=None, residual=None, out=None, out_dtype=None):
+    """Y = activation((A W^T) * a_scale[:, None] * w_scale + bias) + residual, accumulated in fp32.
+
+    A: [..., K], W: [N, K] (a Linear layer's layout), both e4m3 codes, float16 or bfloat16. a_scale: one fp32 entry a row of A
+    (A's leading shape) or one in all; w_scale: [N] or one in all. bias: [N], float32, float16 or bfloat16. activation: as in
+    `quantize_rows`. residual: the output's shape and type; it may be `out`. Output type: out's, or out_dtype, or the
+    residual's, or A's (bfloat16 for codes).
+
+    Operands whose rows do not start at multiples of 16 bytes are copied into such rows first: keep weights in a
+    `PreparedLinear`, codes in tensors from `empty_codes` or the quantisers."""
+    _tensor(A, "A")
+    _tensor(W, "W", A)
+    code = OPERAND_TYPES.get(A.dtype)
+    if code is None or W.dtype != A.dtype:
+        raise TypeError("A and W must both be float8_e4m3fn, float16 or bfloat16, got %s and %s" % (A.dtype, W.dtype))
+    if A.dim() < 1 or W.dim() != 2 or A.shape[-1] != W.shape[1]:
+        raise ValueError("matmul_scaled: A must be [..., K] and W [N, K], got %s and %s" % (tuple(A.shape), tuple(W.shape)))
+    K, N = A.shape[-1], W.shape[0]
+    if K == 0:
+        raise ValueError("matmul_scaled: K must be at least 1")
+    act = _act(activation)
+    M = A.numel() // K
+    shape = A.shape[:-1] + (N,)
+    if out is None:
+        dtype = out_dtype if out_dtype is not None else residual.dtype if residual is not None else \
+            torch.bfloat16 if code == TYPE_E4M3 else A.dtype
+        if dtype not in FLOAT_TYPES:
+            raise TypeError("matmul_scaled: the output must be float32, float16 or bfloat16, not %s" % dtype)
+        out = torch.empty(shape, device=A.device, dtype=dtype)
+    elif out_dtype is not None and out_dtype != out.dtype:
+        raise TypeError("matmul_scaled: out is %s, not %s" % (out.dtype, out_dtype))
+    ytype = _float_type(out, "out")
+    ldy = _output_rows(out, "out", shape, out.dtype, A)
+    rr, ldr = None, 0
+    if residual is not None:
+        _tensor(residual, "residual", A)
+        if residual.dtype != out.dtype or residual.shape != shape:
+            raise ValueError("matmul_scaled: residual must have the output's shape and type")
+        rr, ldr = _input_rows(residual)
+        if ldr < N and M > 1:
+            rr = residual.contiguous()
+            ldr = N
+    btype = 0
+    if bias is not None:
+        _tensor(bias, "bias", A)
+        btype = _float_type(bias, "bias")
+        if bias.shape != (N,):
+            raise ValueError("matmul_scaled: bias must be [%d]" % N)
+        bias = bias.contiguous()
+    a_scale, sa = _scale_operand(a_scale, "a_scale", M, A)
+    w_scale, sw = _scale_operand(w_scale, "w_scale", N, A)
+    A, lda = _operand(A, "A", code, A)
+    W, ldw = _operand(W, "W", code, A)
+    d = GemmScaledDesc(M, N, K, lda, ldw, ldy, ldr, sa, sw, code, btype, ytype, act)
+    _call(_lib.load().b200_gemm_scaled, A.get_device(), ctypes.byref(d), A.data_ptr(), W.data_ptr(),
+          None if a_scale is None else a_scale.data_ptr(), None if w_scale is None else w_scale.data_ptr(),
+          None if bias is None else bias.data_ptr(), None if rr is None else rr.data_ptr(), out.data_ptr())
+    return out
+
+
+class PreparedLinear:
+    """A linear layer whose weight is brought into the product's layout once: e4m3 codes with one scale an output (the
+    default), or float16 / bfloat16.
+
+    weight: [N, K], float32, float16 or bfloat16, on a CUDA device. Calls take activations in any of these types and, for
+    an e4m3 layer, quantise their rows; or e4m3 codes with `a_scale`, as the quantisers return them."""
+
+    def __init__(self, weight, bias=None, *, activation=None, dtype=E4M3):
+        _tensor(weight, "weight")
+        _float_type(weight, "weight")
+        if weight.dim() != 2 or 0 in weight.shape:
+            raise ValueError("PreparedLinear: weight must be [N, K]")
+        if dtype not in OPERAND_TYPES:
+            raise TypeError("PreparedLinear: dtype must be float8_e4m3fn, float16 or bfloat16")
+        _act(activation)
+        self.N, self.K = weight.shape
+        self.activation, self.dtype = activation, dtype
+        if bias is not None:
+            _tensor(bias, "bias", weight)
+            _float_type(bias, "bias")
+            if bias.shape != (self.N,):
+                raise ValueError("PreparedLinear: bias must be [%d]" % self.N)
+            bias = bias.contiguous()
+        self.bias = bias
+        if dtype == E4M3:
+            self.weight, self.w_scale = quantize_rows(weight)
+        else:
+            pitch = -(-self.K // 8) * 8
+            self.weight = torch.empty(self.N, pitch, device=weight.device, dtype=dtype)[:, :self.K]
+            self.weight.copy_(weight)
+            self.w_scale = None
+
+    def __call__(self, x, *, a_scale=None, residual=None, out=None, out_dtype=None):
+        """x: [..., K]. Returns activation(x W^T + bias) + residual in out's type, or out_dtype, or the residual's, or x's
+        (bfloat16 for codes)."""
+        if isinstance(x, torch.Tensor) and x.dtype in FLOAT_TYPES:
+            if out is None and out_dtype is None and residual is None:
+                out_dtype = x.dtype
+            if self.dtype == E4M3:
+                if a_scale is not None:
+                    raise ValueError("PreparedLinear: a_scale belongs to e4m3 codes")
+                x, a_scale = quantize_rows(x)
+            elif x.dtype != self.dtype:
+                x = x.to(self.dtype)
+        elif self.dtype == E4M3 and isinstance(x, torch.Tensor) and x.dtype == E4M3 and a_scale is None:
+            raise ValueError("PreparedLinear: e4m3 codes need their a_scale")
+        return matmul_scaled(x, self.weight, a_scale=a_scale, w_scale=self.w_scale, bias=self.bias,
+                             activation=self.activation, residual=residual, out=out, out_dtype=out_dtype)

@@ -12,7 +12,8 @@ import torch
 from . import _lib
 from ._lib import (ADD, DIV, EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RELU, EPI_BIAS_RESIDUAL, EPI_NONE, EPI_SCALE, ERF,
                    GELU, MATH_MODES, MUL, POW, RELU, SQRT, SUB, AttentionDesc, ConvDesc, GemmDesc, check)  # noqa: F401
-from .lowbit import empty_codes, quantize_rows, rmsnorm, rmsnorm_quantize  # noqa: F401 - typed tensors, 8-bit rows
+from .lowbit import (PreparedLinear, empty_codes, matmul_scaled, quantize_rows, rmsnorm,  # noqa: F401
+                     rmsnorm_quantize)
 
 default_math_mode = "fp32x3"  # "fp32x3" | "tf32" | "bf16" | "fp32"; overridable per call
 

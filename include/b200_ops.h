@@ -302,6 +302,23 @@ typedef struct b200_quantize_desc {
 B200_API int b200_quantize_rows(void *stream, const b200_quantize_desc *desc, const void *x, const void *gate, void *q,
                                 float *scale);
 
+/* Matrix product with bias, activation and residual in its epilogue, on typed operands:
+ *   Y[m, n] = act(a_scale[m] * w_scale[n] * sum_k A[m, k] * W[n, k] + bias[n]) + residual[m, n]
+ * A is [M, K] and W is [N, K] (a Linear layer's layout), both of `type`: B200_TYPE_E4M3, F16 or BF16. Sums in fp32. a_scale
+ * and w_scale (fp32, NULL = 1) have one entry a row (step 1) or one for all rows (step 0). bias: N adjacent entries of
+ * bias_type (F32 / F16 / BF16) or NULL. Y and residual (NULL = none; its rows ldr apart, it may be Y itself) are of y_type.
+ * A and W are read by TMA: their bases must be 16-byte aligned and their row strides multiples of 16 bytes (K itself may be
+ * any length); otherwise the call returns B200_EUNSUPPORTED. 1 <= K. */
+typedef struct b200_gemm_scaled_desc {
+  int64_t M, N, K;
+  int64_t lda, ldw, ldy, ldr;
+  int32_t a_scale_step, w_scale_step;
+  int32_t type, bias_type, y_type;
+  int32_t activation;
+} b200_gemm_scaled_desc;
+B200_API int b200_gemm_scaled(void *stream, const b200_gemm_scaled_desc *desc, const void *A, const void *W,
+                              const float *a_scale, const float *w_scale, const void *bias, const void *residual, void *Y);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from dace_onnx_b200 import _lib, ops
-from dace_onnx_b200._lib import QuantizeDesc, RmsnormDesc
+from dace_onnx_b200._lib import GemmScaledDesc, QuantizeDesc, RmsnormDesc
 from dace_onnx_b200.lowbit import _row_stride
 
 P = ctypes.c_void_p(256)  # never read: the calls below are refused
@@ -61,3 +61,30 @@ def test_row_strides():
     assert _row_stride(t.transpose(1, 2)) is None   # elements of a row apart
     assert _row_stride(t[0, 0].expand(3, 8)) == 0
     assert _row_stride(torch.zeros(5)) == 5 and _row_stride(torch.zeros(3, 1).t()) == 3
+
+
+@pytest.mark.parametrize("change,args,code", [
+    (dict(M=-1), {}, _lib.EINVAL), (dict(N=-1), {}, _lib.EINVAL), (dict(K=0), {}, _lib.EINVAL), (dict(type=0), {}, _lib.EINVAL),
+    (dict(y_type=3), {}, _lib.EINVAL), (dict(bias_type=3), {}, _lib.EINVAL), (dict(activation=5), {}, _lib.EINVAL),
+    (dict(a_scale_step=2), {}, _lib.EINVAL), (dict(w_scale_step=-1), {}, _lib.EINVAL), (dict(lda=16), {}, _lib.EINVAL),
+    (dict(ldw=16), {}, _lib.EINVAL), (dict(ldy=8), {}, _lib.EINVAL), (dict(ldr=8), {}, _lib.EINVAL),
+    (dict(lda=33), {}, _lib.EUNSUPPORTED), (dict(ldw=40), {}, _lib.EUNSUPPORTED), (dict(M=1 << 31), {}, _lib.EUNSUPPORTED),
+    ({}, dict(A=ctypes.c_void_p(264)), _lib.EUNSUPPORTED), ({}, dict(W=ctypes.c_void_p(257)), _lib.EUNSUPPORTED),
+    ({}, dict(A=None), _lib.EINVAL), ({}, dict(W=None), _lib.EINVAL), ({}, dict(Y=None), _lib.EINVAL),
+    (dict(M=0), dict(A=None), _lib.OK), (dict(N=0), dict(W=None), _lib.OK)])
+def test_gemm_scaled_refusals(change, args, code):
+    d = GemmScaledDesc(4, 16, 32, 32, 32, 16, 16, 1, 1, 3, 0, 0, 0)
+    for k, v in change.items():
+        setattr(d, k, v)
+    a = dict(A=P, W=P, a_scale=P, w_scale=P, bias=P, residual=P, Y=P)
+    a.update(args)
+    assert _lib.load().b200_gemm_scaled(None, ctypes.byref(d), *a.values()) == code
+    assert _lib.load().b200_gemm_scaled(None, None, P, P, P, P, P, P, P) == _lib.EINVAL
+
+
+def test_products_of_cpu_tensors_are_refused():
+    x = torch.zeros(2, 16, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="no CPU path"):
+        ops.matmul_scaled(x, x)
+    with pytest.raises(ValueError, match="no CPU path"):
+        ops.PreparedLinear(x)
