@@ -13,7 +13,7 @@
 //          change places: 128 rows of W are the TMEM lanes and NT rows of A the columns, so that a single token fills
 //          the tensor core's wide side with weights. K is split over the CTAs of a cluster (at most 8), whose partial
 //          sums meet in distributed shared memory in a fixed order (the same bits every time, no workspace). Lanes of
-//          a warp hold neighbouring columns of Y, so its stores are dense at any alignment: it also takes outputs
+//          a warp write neighbouring columns of Y, so its stores are dense at any alignment: it also takes outputs
 //          whose rows the pair kernel's vector accesses cannot address.
 //
 // The tensor core adds into its fp32 accumulator with truncation, an error that grows with the number of additions. For
@@ -45,7 +45,7 @@ struct ScaledParams {
   uint32_t idesc;
   int a_scale_step, w_scale_step;
   int bias_type, activation;
-  int vec;                                        // widest access to rows of Y and residual: 32 or 16 bytes (pair)
+  int vec;                                        // widest access to rows of Y and residual: 32, 16, 8 or 0 bytes
   int64_t ldy, ldr;
   const float *a_scale, *w_scale;
   const void *bias, *residual;
@@ -68,8 +68,8 @@ __device__ __forceinline__ float a_scale_at(const ScaledParams &p, int64_t m) {
   return p.a_scale ? __ldg(p.a_scale + m * p.a_scale_step) : 1.f;
 }
 
-// 32 bytes of a row, in one access or two
-__device__ __forceinline__ void load32(const void *p, int vec, uint32_t (&w)[8]) {
+// 32 bytes of a row of the residual, in one access or two
+__device__ __forceinline__ void load32(const void *p, int vec, uint32_t *w) {
   if (vec == 32) {
     asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
@@ -80,78 +80,116 @@ __device__ __forceinline__ void load32(const void *p, int vec, uint32_t (&w)[8])
     w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
   }
 }
-__device__ __forceinline__ void store32(void *p, int vec, const uint32_t (&w)[8]) {
-  if (vec == 32) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                 ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+
+// Pair kernel: 64 bytes of outputs of one row, held by one thread (32 of a 16-bit type, 16 of fp32), to shared memory. sw,
+// bs: scales and biases of these columns in shared memory (broadcast reads). r: the row's residual (RES) or null; cols: how
+// many of the outputs exist (the others are computed from zeros and cut off by the store). row: the row's 64 bytes; flip: the
+// exchange of its 16-byte pieces.
+template <typename OUT>
+constexpr int kBlockCols = 64 / (int)sizeof(OUT);
+template <typename OUT, int ACT, bool RES>
+__device__ __forceinline__ void finish_block_t(const ScaledParams &p, const float *v, float sa, const float *sw,
+                                               const float *bs, const OUT *r, int cols, uint32_t row, uint32_t flip) {
+  constexpr int B = kBlockCols<OUT>, C = 16 / (int)sizeof(OUT);  // outputs of the block, of 16 bytes
+  const Pair sa2 = both(sa);
+  uint32_t add[RES ? 16 : 1];
+  if (RES) {
+    if (r && cols >= B) {
+      load32(r, p.vec, add);
+      load32(r + B / 2, p.vec, add + 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if constexpr (sizeof(OUT) == 4) {
+          add[i] = r && i < cols ? __float_as_uint(to_f32<OUT>(r[i])) : 0u;
+        } else {
+          add[i] = pack2<OUT>(r && 2 * i < cols ? to_f32<OUT>(r[2 * i]) : 0.f,
+                              r && 2 * i + 1 < cols ? to_f32<OUT>(r[2 * i + 1]) : 0.f);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < C; i += 4) {
+      const int j = g * C + i;
+      const float4 s = *reinterpret_cast<const float4 *>(sw + j), b = *reinterpret_cast<const float4 *>(bs + j);
+      Pair lo = activate2_t<ACT>(fma2(Pair(v[j], v[j + 1]) * sa2, Pair(s.x, s.y), Pair(b.x, b.y)));
+      Pair hi = activate2_t<ACT>(fma2(Pair(v[j + 2], v[j + 3]) * sa2, Pair(s.z, s.w), Pair(b.z, b.w)));
+      float o[4];
+      if (RES) {
+        if constexpr (sizeof(OUT) == 4) {
+          lo = lo + Pair(__uint_as_float(add[j]), __uint_as_float(add[j + 1]));
+          hi = hi + Pair(__uint_as_float(add[j + 2]), __uint_as_float(add[j + 3]));
+        } else {
+          float x, y;
+          unpack2<OUT>(add[j / 2], x, y);
+          lo = lo + Pair(x, y);
+          unpack2<OUT>(add[j / 2 + 1], x, y);
+          hi = hi + Pair(x, y);
+        }
+      }
+      lo.get(o[0], o[1]);
+      hi.get(o[2], o[3]);
+      if constexpr (sizeof(OUT) == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = __float_as_uint(o[k]);
+      } else {
+        w[i / 2] = pack2<OUT>(o[0], o[1]);
+        w[i / 2 + 1] = pack2<OUT>(o[2], o[3]);
+      }
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((g ^ flip) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3])
                  : "memory");
-  } else {
-    static_cast<uint4 *>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    static_cast<uint4 *>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+template <typename OUT, bool RES>
+__device__ __forceinline__ void finish_block(const ScaledParams &p, const float *v, float sa, const float *sw,
+                                             const float *bs, const OUT *r, int cols, uint32_t row, uint32_t flip) {
+  switch (p.activation) {  // uniform for the launch
+    case B200_ACT_RELU: finish_block_t<OUT, B200_ACT_RELU, RES>(p, v, sa, sw, bs, r, cols, row, flip); break;
+    case B200_ACT_GELU: finish_block_t<OUT, B200_ACT_GELU, RES>(p, v, sa, sw, bs, r, cols, row, flip); break;
+    case B200_ACT_GELU_TANH: finish_block_t<OUT, B200_ACT_GELU_TANH, RES>(p, v, sa, sw, bs, r, cols, row, flip); break;
+    case B200_ACT_SILU: finish_block_t<OUT, B200_ACT_SILU, RES>(p, v, sa, sw, bs, r, cols, row, flip); break;
+    default: finish_block_t<OUT, B200_ACT_NONE, RES>(p, v, sa, sw, bs, r, cols, row, flip);
   }
 }
 
-// Pair kernel: 32 neighbouring outputs of one row, held by one thread. sw, bs: scales and biases of these columns in
-// shared memory (broadcast reads). cols: how many of the 32 exist.
-template <typename OUT, int ACT>
-__device__ __forceinline__ void finish32_t(const ScaledParams &p, const float (&v)[32], float sa, const float *sw,
-                                           const float *bs, const OUT *r, OUT *y, int cols) {
-  constexpr int G = 32 / (int)sizeof(OUT);  // outputs of 32 bytes
-  if (cols >= 32) {
-#pragma unroll
-    for (int g = 0; g < 32; g += G) {
-      float o[G];
-#pragma unroll
-      for (int i = 0; i < G; i += 4) {
-        const float4 s = *reinterpret_cast<const float4 *>(sw + g + i), b = *reinterpret_cast<const float4 *>(bs + g + i);
-        o[i] = activate_t<ACT>(fmaf(v[g + i] * sa, s.x, b.x));
-        o[i + 1] = activate_t<ACT>(fmaf(v[g + i + 1] * sa, s.y, b.y));
-        o[i + 2] = activate_t<ACT>(fmaf(v[g + i + 2] * sa, s.z, b.z));
-        o[i + 3] = activate_t<ACT>(fmaf(v[g + i + 3] * sa, s.w, b.w));
-      }
-      uint32_t w[8];
-      if (r) {
-        load32(r + g, p.vec, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if constexpr (sizeof(OUT) == 4) {
-            o[i] += __uint_as_float(w[i]);
-          } else {
-            float lo, hi;
-            unpack2<OUT>(w[i], lo, hi);
-            o[2 * i] += lo;
-            o[2 * i + 1] += hi;
-          }
+// The loading and the issuing warp run converged, with one elected lane issuing: loop variables, addresses and
+// descriptors then live in uniform registers. (With a single lane in a branch of its own each of them had to be moved there for
+// every instruction: 170 clk per TMA load and 85 per MMA, against 128 clk that an MMA takes.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
+// mbar_wait by a converged warp; the answer is the same in all lanes.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int *abort_flag, unsigned *status,
+                                               unsigned code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const long long t0 = clock64();
+  for (uint32_t it = 1;; ++it) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((it & 0xffu) == 0) {
+      const bool late = clock64() - t0 > kWaitCycleBudget;
+      if (__any_sync(0xffffffffu, late || *abort_flag)) {
+        if (late) {
+          *abort_flag = 1;
+          atomicOr(status, code);
         }
+        return false;
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if constexpr (sizeof(OUT) == 4) w[i] = __float_as_uint(o[i]);
-        else w[i] = pack2<OUT>(o[2 * i], o[2 * i + 1]);
-      }
-      store32(y + g, p.vec, w);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < cols) {
-        float o = activate_t<ACT>(fmaf(v[i] * sa, sw[i], bs[i]));
-        if (r) o += to_f32<OUT>(r[i]);
-        y[i] = from_f32<OUT>(o);
-      }
   }
 }
-template <typename OUT>
-__device__ __forceinline__ void finish32(const ScaledParams &p, const float (&v)[32], float sa, const float *sw,
-                                         const float *bs, const OUT *r, OUT *y, int cols) {
-  switch (p.activation) {  // uniform for the launch
-    case B200_ACT_RELU: finish32_t<OUT, B200_ACT_RELU>(p, v, sa, sw, bs, r, y, cols); break;
-    case B200_ACT_GELU: finish32_t<OUT, B200_ACT_GELU>(p, v, sa, sw, bs, r, y, cols); break;
-    case B200_ACT_GELU_TANH: finish32_t<OUT, B200_ACT_GELU_TANH>(p, v, sa, sw, bs, r, y, cols); break;
-    case B200_ACT_SILU: finish32_t<OUT, B200_ACT_SILU>(p, v, sa, sw, bs, r, y, cols); break;
-    default: finish32_t<OUT, B200_ACT_NONE>(p, v, sa, sw, bs, r, y, cols);
-  }
-}
+__device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
 
 __device__ __forceinline__ void teardown_after_abort(int aborted) {
   // copies may still be in flight after a wait gave up: leave them time before the shared memory goes
@@ -166,16 +204,15 @@ __device__ __forceinline__ void teardown_after_abort(int aborted) {
 // ---------------------------------------------------------------------------------------------
 template <int BN>
 struct PairCfg {
-  static constexpr int kBHalfBytes = BN / 2 * kRowBytes;   // each CTA loads half of the tile's rows of W
-  static constexpr int kKbPerStage = 2;                    // one wait and one commit per eight MMAs
-  static constexpr int kStageBytes = kKbPerStage * (kTileBytes + kBHalfBytes);
-  static constexpr int kStages = (192 * 1024) / kStageBytes;
+  static constexpr int kStageBytes = kTileBytes + BN / 2 * kRowBytes;  // 128 rows of A, half of the tile's rows of W
+  static constexpr int kStages = (160 * 1024) / kStageBytes;
   static constexpr int kTmemCols = 2 * BN;
   static constexpr int kColsPerWarp = BN / 4;              // four warps on each quarter of the lanes
   static constexpr int kEpilogueWarps = 16;
   static constexpr int kThreads = 32 * (2 + kEpilogueWarps);
-  static constexpr int kStagingBytes = kEpilogueWarps * kColsPerWarp * 2 * 4;
-  static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256 + kStagingBytes;
+  static constexpr int kStoreBytes = 32 * 64;              // a warp's block of outputs: 32 rows of 64 bytes
+  static constexpr int kVectorBytes = kColsPerWarp * 2 * 4;  // a warp's scales and biases
+  static constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * (kStoreBytes + kVectorBytes) + 1024 + 256;
 };
 
 // Tiles in groups of eight row tiles, column tiles across a group: the ~74 tiles in flight then share about 8 + 9 tile
@@ -193,15 +230,16 @@ __device__ __forceinline__ void tile_at(const ScaledParams &p, int64_t tile, int
 template <bool F8, typename OUT, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::kThreads, 1)
 scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
-                   const ScaledParams p) {
+                   const __grid_constant__ CUtensorMap map_y, const ScaledParams p) {
   using C = PairCfg<BN>;
   constexpr bool kChunked = std::is_same<OUT, float>::value;
   constexpr int kStages = C::kStages;
   constexpr int kKbElems = F8 ? 128 : 64;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  float *staging = reinterpret_cast<float *>(smem + kStages * C::kStageBytes);
-  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kStages * C::kStageBytes + C::kStagingBytes);
+  uint8_t *store_smem = smem + kStages * C::kStageBytes;
+  uint8_t *vector_smem = store_smem + C::kEpilogueWarps * C::kStoreBytes;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(vector_smem + C::kEpilogueWarps * C::kVectorBytes);
   const uint32_t bar_full = smem_u32(bars);
   const uint32_t bar_empty = bar_full + 8 * kStages;
   const uint32_t bar_tfull = bar_empty + 8 * kStages;
@@ -209,7 +247,7 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   const uint32_t smem_base = smem_u32(smem);
   const uint32_t rank = cluster_ctarank();
   const int64_t pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
@@ -239,72 +277,67 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   volatile int *abort_flag = &s_abort;
 
   if (warp == 0) {
-    if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      const uint32_t full_pair0 = map_to_cta(bar_full, 0);
-      for (int64_t tile = pair; tile < num_tiles && ok; tile += num_pairs) {
-        int m_t, n_t;
-        tile_at(p, tile, m_t, n_t);
-        const int row_a = m_t * 256 + (int)rank * 128;
-        const int row_w = n_t * BN + (int)rank * (BN / 2);
-        for (int kb = 0; kb < p.num_kb; kb += C::kKbPerStage) {
-          if (!(ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 1u))) break;
-          // a K-block past the end of K is filled with zeros
-          const uint32_t stage = smem_base + s * C::kStageBytes;
-          if (rank == 0) mbar_expect_tx(bar_full + 8 * s, 2 * C::kStageBytes);
-#pragma unroll
-          for (int h = 0; h < C::kKbPerStage; ++h) {
-            const uint32_t a_dst = stage + h * kTileBytes;
-            const uint32_t w_dst = stage + C::kKbPerStage * kTileBytes + h * C::kBHalfBytes;
-            const int k0 = (kb + h) * kKbElems;
-            if (rank == 0) {
-              tma_load_2d(a_dst, &map_a, bar_full + 8 * s, k0, row_a);
-              tma_load_2d(w_dst, &map_w, bar_full + 8 * s, k0, row_w);
-            } else {
-              tma_load_2d_pair(a_dst, &map_a, full_pair0 + 8 * s, k0, row_a);
-              tma_load_2d_pair(w_dst, &map_w, full_pair0 + 8 * s, k0, row_w);
-            }
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    const uint32_t full_pair0 = map_to_cta(bar_full, 0);
+    for (int64_t tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+      int m_t, n_t;
+      tile_at(p, tile, m_t, n_t);
+      const int row_a = m_t * 256 + (int)rank * 128;
+      const int row_w = n_t * BN + (int)rank * (BN / 2);
+      for (int kb = 0; kb < p.num_kb; ++kb) {
+        if (!(ok = mbar_wait_warp(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 1u))) break;
+        // one expect_tx, by the even CTA, for the bytes of both: its partner's can arrive only after the stage's previous
+        // phase is complete, because they too wait for the commit that follows it
+        const uint32_t a_dst = smem_base + s * C::kStageBytes, w_dst = a_dst + kTileBytes;
+        if (elect_one()) {
+          if (rank == 0) {
+            mbar_expect_tx(bar_full + 8 * s, 2 * C::kStageBytes);
+            tma_load_2d(a_dst, &map_a, bar_full + 8 * s, kb * kKbElems, row_a);
+            tma_load_2d(w_dst, &map_w, bar_full + 8 * s, kb * kKbElems, row_w);
+          } else {
+            tma_load_2d_pair(a_dst, &map_a, full_pair0 + 8 * s, kb * kKbElems, row_a);
+            tma_load_2d_pair(w_dst, &map_w, full_pair0 + 8 * s, kb * kKbElems, row_w);
           }
-          if (++s == kStages) { s = 0; ph ^= 1; }
         }
+        __syncwarp();
+        if (++s == kStages) { s = 0; ph ^= 1; }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      constexpr uint32_t kStage16 = C::kStageBytes >> 4;
+    if (rank == 0) {
       const uint64_t a_desc0 = make_smem_desc(smem_base, 16, 1024, kLayoutSw128);
-      const uint64_t w_desc0 = make_smem_desc(smem_base + C::kKbPerStage * kTileBytes, 16, 1024, kLayoutSw128);
+      const uint64_t w_desc0 = make_smem_desc(smem_base + kTileBytes, 16, 1024, kLayoutSw128);
       const uint32_t idesc = p.idesc;
-      const int chunk = kChunked ? kChunkKb : p.num_kb + C::kKbPerStage;  // a multiple of the stage, or everything
+      const int chunk = kChunked ? kChunkKb : p.num_kb;
       int s = 0, acc = 0;
       uint32_t ph = 0, acc_ph = 0;
       bool ok = true;
       for (int64_t tile = pair; tile < num_tiles && ok; tile += num_pairs) {
         for (int kb0 = 0; kb0 < p.num_kb && ok; kb0 += chunk) {
-          if (!(ok = mbar_wait(bar_tempty + 8 * acc, acc_ph ^ 1, abort_flag, p.status, 2u))) break;
+          if (!(ok = mbar_wait_warp(bar_tempty + 8 * acc, acc_ph ^ 1, abort_flag, p.status, 2u))) break;
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
           const int kb_end = min(kb0 + chunk, p.num_kb);
-          for (int kb = kb0; kb < kb_end; kb += C::kKbPerStage) {
-            if (!(ok = mbar_wait(bar_full + 8 * s, ph, abort_flag, p.status, 4u))) break;
+          for (int kb = kb0; kb < kb_end; ++kb) {
+            if (!(ok = mbar_wait_warp(bar_full + 8 * s, ph, abort_flag, p.status, 4u))) break;
             tc_fence_after();
-            const uint64_t a_d = a_desc0 + (uint32_t)s * kStage16, w_d = w_desc0 + (uint32_t)s * kStage16;
-#pragma unroll
-            for (int h = 0; h < C::kKbPerStage; ++h)
+            const uint64_t a_d = a_desc0 + (uint32_t)s * (C::kStageBytes >> 4);
+            const uint64_t w_d = w_desc0 + (uint32_t)s * (C::kStageBytes >> 4);
+            if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < kMmasPerKb; ++k) {
-                const uint64_t a = a_d + h * (kTileBytes >> 4) + 2 * k, w = w_d + h * (C::kBHalfBytes >> 4) + 2 * k;
-                const uint32_t accumulate = (h > 0 || k > 0 || kb > kb0) ? 1u : 0u;
-                if (F8) umma_f8_pair(d_tmem, a, w, idesc, accumulate);
-                else umma_bf16_pair(d_tmem, a, w, idesc, accumulate);
+                const uint32_t accumulate = (k > 0 || kb > kb0) ? 1u : 0u;
+                if (F8) umma_f8_pair(d_tmem, a_d + 2 * k, w_d + 2 * k, idesc, accumulate);
+                else umma_bf16_pair(d_tmem, a_d + 2 * k, w_d + 2 * k, idesc, accumulate);
               }
-            umma_commit_pair_both(bar_empty + 8 * s, 3);
+              umma_commit_pair_both(bar_empty + 8 * s, 3);
+              if (kb + 1 == kb_end) umma_commit_pair_both(bar_tfull + 8 * acc, 3);
+            }
+            __syncwarp();
             if (++s == kStages) { s = 0; ph ^= 1; }
           }
-          if (!ok) break;
-          umma_commit_pair_both(bar_tfull + 8 * acc, 3);
           if (++acc == 2) { acc = 0; acc_ph ^= 1; }
         }
       }
@@ -312,16 +345,21 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   } else {
     const int ew = warp - 2, quarter = warp & 3;
     const int col0 = (ew >> 2) * C::kColsPerWarp;
-    float *sw = staging + ew * (2 * C::kColsPerWarp), *bs = sw + C::kColsPerWarp;
+    float *sw = reinterpret_cast<float *>(vector_smem + ew * C::kVectorBytes), *bs = sw + C::kColsPerWarp;
+    // the block of outputs on its way to memory: rows of 64 bytes whose 16-byte pieces are exchanged as the 64-byte
+    // swizzle of map_y has them, so that a warp's 16-byte accesses meet no bank twice
+    const uint32_t block = smem_u32(store_smem + ew * C::kStoreBytes);
+    const uint32_t my_row = block + lane * 64, flip = (lane >> 1) & 3;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + col0;
     const int chunks = kChunked ? (p.num_kb + kChunkKb - 1) / kChunkKb : 1;
+    constexpr int B = kBlockCols<OUT>;
     int acc = 0;
     uint32_t acc_ph = 0;
     bool ok = true;
     for (int64_t tile = pair; tile < num_tiles && ok; tile += num_pairs) {
       int m_t, n_t;
       tile_at(p, tile, m_t, n_t);
-      const int64_t m = (int64_t)m_t * 256 + (int)rank * 128 + quarter * 32 + lane;
+      const int64_t m0 = (int64_t)m_t * 256 + (int)rank * 128 + quarter * 32, m = m0 + lane;
       const int64_t n0 = (int64_t)n_t * BN + col0;
       // this warp's columns: scales and biases to shared memory, while the MMAs run
       __syncwarp();
@@ -333,16 +371,27 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       __syncwarp();
       const bool row_in = m < p.M;
       const float sa = row_in ? a_scale_at(p, m) : 0.f;
-      OUT *y = static_cast<OUT *>(p.Y) + m * p.ldy + n0;
-      const OUT *r = p.residual ? static_cast<const OUT *>(p.residual) + m * p.ldr + n0 : nullptr;
-      auto emit = [&](const float (&v)[32], int c) {
+      const OUT *r = p.residual && row_in ? static_cast<const OUT *>(p.residual) + m * p.ldr + n0 : nullptr;
+      // 64 bytes of each of the warp's rows, from the accumulators v of columns c..c+B-1
+      auto emit = [&](const float *v, int c) {
         const int64_t left = p.N - n0 - c;
-        if (row_in && left > 0) finish32<OUT>(p, v, sa, sw + c, bs + c, r ? r + c : nullptr, y + c, left < 32 ? (int)left : 32);
+        if (left <= 0 || m0 >= p.M) return;  // uniform
+        const int cols = left < B ? (int)left : B;
+        if (lane == 0) bulk_wait_read();  // the previous block has left
+        __syncwarp();
+        if (p.residual) finish_block<OUT, true>(p, v, sa, sw + c, bs + c, r ? r + c : nullptr, cols, my_row, flip);
+        else finish_block<OUT, false>(p, v, sa, sw + c, bs + c, nullptr, cols, my_row, flip);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&map_y, block, (int)(n0 + c), (int)m0);
+          bulk_commit();
+        }
       };
       if (kChunked) {
-        float sum[C::kColsPerWarp / 32][32] = {};
+        float sum[C::kColsPerWarp] = {};
         for (int ch = 0; ch < chunks; ++ch) {
-          if (!(ok = mbar_wait(bar_tfull + 8 * acc, acc_ph, abort_flag, p.status, 8u))) break;
+          if (!(ok = mbar_wait_warp(bar_tfull + 8 * acc, acc_ph, abort_flag, p.status, 8u))) break;
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < C::kColsPerWarp; c += 16) {
@@ -350,7 +399,7 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             tmem_ld16(lane_addr + (uint32_t)(acc * BN + c), t);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) sum[c / 32][c % 32 + j] += __uint_as_float(t[j]);
+            for (int j = 0; j < 16; ++j) sum[c + j] += __uint_as_float(t[j]);
           }
           tc_fence_before();
           __syncwarp();
@@ -359,15 +408,14 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         }
         if (!ok) break;
 #pragma unroll
-        for (int c = 0; c < C::kColsPerWarp / 32; ++c) emit(sum[c], 32 * c);
+        for (int c = 0; c < C::kColsPerWarp; c += B) emit(sum + c, c);
       } else {
-        if (!(ok = mbar_wait(bar_tfull + 8 * acc, acc_ph, abort_flag, p.status, 8u))) break;
+        if (!(ok = mbar_wait_warp(bar_tfull + 8 * acc, acc_ph, abort_flag, p.status, 8u))) break;
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < C::kColsPerWarp; c += 32) {
           uint32_t t[32];
           float v[32];
-          __syncwarp();
           tmem_ld32(lane_addr + (uint32_t)(acc * BN + c), t);
           tmem_ld_wait();
           if (c + 32 >= C::kColsPerWarp) {
@@ -382,6 +430,7 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         if (++acc == 2) { acc = 0; acc_ph ^= 1; }
       }
     }
+    if (lane == 0) bulk_wait();
   }
 
   // neither CTA may leave while its partner can still signal its barriers or read its shared memory
@@ -415,31 +464,128 @@ struct SplitCfg {
   static_assert(NT * 128 * 4 <= kStages * kStageBytes, "partial sums take the place of the stages");
 };
 
+// Loads from the shared memory of a CTA of the cluster, after a cluster barrier. Not ordered against global accesses, so
+// that those of several rows are in flight together.
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
 
-// Outputs of this CTA: its share of the tile's rows of A (rank, rank + S, ...), for W row n of this thread.
+// Four neighbouring outputs in one access (8 bytes of a 16-bit type, 16 of fp32).
+template <typename OUT>
+__device__ __forceinline__ void load4(const OUT *p, float (&v)[4]) {
+  if constexpr (sizeof(OUT) == 4) {
+    const float4 f = *reinterpret_cast<const float4 *>(p);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    unpack2<OUT>(u.x, v[0], v[1]);
+    unpack2<OUT>(u.y, v[2], v[3]);
+  }
+}
+template <typename OUT>
+__device__ __forceinline__ void store4(OUT *p, const float (&v)[4]) {
+  if constexpr (sizeof(OUT) == 4) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3]));
+}
+
 template <typename OUT, int ACT>
-__device__ __forceinline__ void finish_split_t(const ScaledParams &p, uint32_t partial, int ranks, int rank, int first,
-                                               int step, int64_t m0, int rows, int64_t n) {
-  const float sw = w_scale_at(p, n), bias = bias_at(p, n);
-  uint32_t base[8];
+__device__ __forceinline__ void epilogue4_t(const float4 &v, float sa, const float (&sw)[4], const float (&bs)[4],
+                                            const float (&add)[4], float (&o)[4]) {
+  const Pair sa2 = both(sa);
+  const Pair lo = activate2_t<ACT>(fma2(Pair(v.x, v.y) * sa2, Pair(sw[0], sw[1]), Pair(bs[0], bs[1])));
+  const Pair hi = activate2_t<ACT>(fma2(Pair(v.z, v.w) * sa2, Pair(sw[2], sw[3]), Pair(bs[2], bs[3])));
+  (lo + Pair(add[0], add[1])).get(o[0], o[1]);
+  (hi + Pair(add[2], add[3])).get(o[2], o[3]);
+}
+
+// Outputs of this CTA: its share of the tile's rows of A (rank, rank + RANKS, ...). A warp takes a row of A at a time and
+// the tile's 128 columns of Y: VEC: lane l has columns 4l..4l+3 and one access; otherwise columns l, l+32, l+64, l+96
+// and dense scalar accesses. Eight partial sums (4 to 1 rows) are in flight together.
+template <typename OUT, bool VEC, int RANKS>
+__device__ __forceinline__ void finish_split_t(const ScaledParams &p, uint32_t partial, int rank, int warp, int warps,
+                                               int lane, int64_t m0, int rows, int64_t n0, const float (&sw)[4],
+                                               const float (&bs)[4]) {
+  constexpr int R = RANKS == 8 ? 1 : RANKS == 4 ? 2 : 4;
+  const int64_t left = p.N - n0;
+  auto col = [&](int k) { return VEC ? 4 * lane + k : lane + 32 * k; };
+  OUT *y = static_cast<OUT *>(p.Y) + m0 * p.ldy + n0;
+  const OUT *r = p.residual ? static_cast<const OUT *>(p.residual) + m0 * p.ldr + n0 : nullptr;
+  const bool whole = VEC && col(3) < left;
+  uint32_t base[RANKS];
 #pragma unroll
-  for (int s = 0; s < 8; ++s) base[s] = s < ranks ? map_to_cta(partial, s) : 0u;
-  OUT *y = static_cast<OUT *>(p.Y) + m0 * p.ldy + n;
-  const OUT *r = p.residual ? static_cast<const OUT *>(p.residual) + m0 * p.ldr + n : nullptr;
-#pragma unroll 4
-  for (int t = rank + first * ranks; t < rows; t += step * ranks) {
-    float v = 0.f;
+  for (int s = 0; s < RANKS; ++s) base[s] = map_to_cta(partial, s);
+  for (int j0 = warp; rank + RANKS * j0 < rows; j0 += R * warps) {
+    float4 part[R][RANKS];
+    float add[R][4], sa[R];
 #pragma unroll
-    for (int s = 0; s < 8; ++s)
-      if (s < ranks) v += ld_cluster(base[s] + (uint32_t)t * 512);
-    float o = activate_t<ACT>(fmaf(v * a_scale_at(p, m0 + t), sw, bias));
-    if (r) o += to_f32<OUT>(r[t * p.ldr]);
-    y[t * p.ldy] = from_f32<OUT>(o);
+    for (int i = 0; i < R; ++i) {
+      const int t = rank + RANKS * (j0 + i * warps);
+      if (t >= rows) break;
+#pragma unroll
+      for (int s = 0; s < RANKS; ++s) {
+        if (VEC) {
+          part[i][s] = ld_cluster4(base[s] + t * 512 + lane * 16);
+        } else {
+          const uint32_t q = base[s] + t * 512 + lane * 4;
+          part[i][s] = make_float4(ld_cluster(q), ld_cluster(q + 128), ld_cluster(q + 256), ld_cluster(q + 384));
+        }
+      }
+      sa[i] = a_scale_at(p, m0 + t);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) add[i][k] = 0.f;
+      if (r) {
+        if (whole) {
+          load4<OUT>(r + t * p.ldr + 4 * lane, add[i]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (col(k) < left) add[i][k] = to_f32<OUT>(r[t * p.ldr + col(k)]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int t = rank + RANKS * (j0 + i * warps);
+      if (t >= rows) break;
+      float4 v = part[i][0];
+#pragma unroll
+      for (int s = 1; s < RANKS; ++s) {
+        v.x += part[i][s].x; v.y += part[i][s].y; v.z += part[i][s].z; v.w += part[i][s].w;
+      }
+      float o[4];
+      switch (p.activation) {  // uniform for the launch
+        case B200_ACT_RELU: epilogue4_t<OUT, B200_ACT_RELU>(v, sa[i], sw, bs, add[i], o); break;
+        case B200_ACT_GELU: epilogue4_t<OUT, B200_ACT_GELU>(v, sa[i], sw, bs, add[i], o); break;
+        case B200_ACT_GELU_TANH: epilogue4_t<OUT, B200_ACT_GELU_TANH>(v, sa[i], sw, bs, add[i], o); break;
+        case B200_ACT_SILU: epilogue4_t<OUT, B200_ACT_SILU>(v, sa[i], sw, bs, add[i], o); break;
+        default: epilogue4_t<OUT, B200_ACT_NONE>(v, sa[i], sw, bs, add[i], o);
+      }
+      if (whole) {
+        store4<OUT>(y + t * p.ldy + 4 * lane, o);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (col(k) < left) y[t * p.ldy + col(k)] = from_f32<OUT>(o[k]);
+      }
+    }
+  }
+}
+template <typename OUT, bool VEC>
+__device__ __forceinline__ void finish_split(const ScaledParams &p, uint32_t partial, int ranks, int rank, int warp,
+                                             int warps, int lane, int64_t m0, int rows, int64_t n0, const float (&sw)[4],
+                                             const float (&bs)[4]) {
+  switch (ranks) {  // uniform for the launch
+    case 1: finish_split_t<OUT, VEC, 1>(p, partial, rank, warp, warps, lane, m0, rows, n0, sw, bs); break;
+    case 2: finish_split_t<OUT, VEC, 2>(p, partial, rank, warp, warps, lane, m0, rows, n0, sw, bs); break;
+    case 4: finish_split_t<OUT, VEC, 4>(p, partial, rank, warp, warps, lane, m0, rows, n0, sw, bs); break;
+    default: finish_split_t<OUT, VEC, 8>(p, partial, rank, warp, warps, lane, m0, rows, n0, sw, bs);
   }
 }
 
@@ -462,7 +608,7 @@ scaled_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   const uint32_t smem_base = smem_u32(smem);
   const int rank = (int)cluster_ctarank();
   const int64_t tile = blockIdx.x / ranks;
@@ -490,62 +636,74 @@ scaled_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   tc_fence_after();
   const uint32_t tmem_base = s_tmem_base;
   volatile int *abort_flag = &s_abort;
+  const int64_t m0 = (int64_t)m_t * NT, n0 = (int64_t)n_t * 128;
+  const bool vec = p.vec >= 4 * (int)sizeof(OUT);
+  float sw[4], bs[4];  // scales and biases of this lane's columns of Y, loaded while the operands arrive
 
   if (warp == 0) {
-    if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 0;
-      for (int kb = kb_begin; kb < kb_end; ++kb) {
-        if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 1u)) break;
-        const uint32_t stage = smem_base + s * C::kStageBytes;
+    int s = 0;
+    uint32_t ph = 0;
+    for (int kb = kb_begin; kb < kb_end; ++kb) {
+      if (!mbar_wait_warp(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 1u)) break;
+      const uint32_t stage = smem_base + s * C::kStageBytes;
+      if (elect_one()) {
         mbar_expect_tx(bar_full + 8 * s, C::kStageBytes);
         tma_load_2d(stage, &map_w, bar_full + 8 * s, kb * kKbElems, n_t * 128);
         tma_load_2d(stage + kTileBytes, &map_a, bar_full + 8 * s, kb * kKbElems, m_t * NT);
-        if (++s == kStages) { s = 0; ph ^= 1; }
       }
+      __syncwarp();
+      if (++s == kStages) { s = 0; ph ^= 1; }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint64_t w_desc0 = make_smem_desc(smem_base, 16, 1024, kLayoutSw128);
-      const uint64_t a_desc0 = make_smem_desc(smem_base + kTileBytes, 16, 1024, kLayoutSw128);
-      const int chunk = kChunked ? kChunkKb : p.num_kb;
-      int s = 0, acc = 0;
-      uint32_t ph = 0, acc_ph = 0;
-      bool ok = true;
-      for (int kb0 = kb_begin; kb0 < kb_end && ok; kb0 += chunk) {
-        if (!(ok = mbar_wait(bar_tempty + 8 * acc, acc_ph ^ 1, abort_flag, p.status, 2u))) break;
+    const uint64_t w_desc0 = make_smem_desc(smem_base, 16, 1024, kLayoutSw128);
+    const uint64_t a_desc0 = make_smem_desc(smem_base + kTileBytes, 16, 1024, kLayoutSw128);
+    const uint32_t idesc = p.idesc;
+    const int chunk = kChunked ? kChunkKb : p.num_kb;
+    int s = 0, acc = 0;
+    uint32_t ph = 0, acc_ph = 0;
+    bool ok = true;
+    for (int kb0 = kb_begin; kb0 < kb_end && ok; kb0 += chunk) {
+      if (!(ok = mbar_wait_warp(bar_tempty + 8 * acc, acc_ph ^ 1, abort_flag, p.status, 2u))) break;
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + (uint32_t)(acc * C::kAccCols);
+      const int end = min(kb0 + chunk, kb_end);
+      for (int kb = kb0; kb < end; ++kb) {
+        if (!(ok = mbar_wait_warp(bar_full + 8 * s, ph, abort_flag, p.status, 4u))) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * C::kAccCols);
-        for (int kb = kb0; kb < min(kb0 + chunk, kb_end); ++kb) {
-          if (!(ok = mbar_wait(bar_full + 8 * s, ph, abort_flag, p.status, 4u))) break;
-          tc_fence_after();
-          const uint64_t w_d = w_desc0 + (uint32_t)s * (C::kStageBytes >> 4);
-          const uint64_t a_d = a_desc0 + (uint32_t)s * (C::kStageBytes >> 4);
+        const uint64_t w_d = w_desc0 + (uint32_t)s * (C::kStageBytes >> 4);
+        const uint64_t a_d = a_desc0 + (uint32_t)s * (C::kStageBytes >> 4);
+        if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < kMmasPerKb; ++k) {
             const uint32_t accumulate = (k > 0 || kb > kb0) ? 1u : 0u;
-            if (F8) umma_f8(d_tmem, w_d + 2 * k, a_d + 2 * k, p.idesc, accumulate);
-            else umma_bf16(d_tmem, w_d + 2 * k, a_d + 2 * k, p.idesc, accumulate);
+            if (F8) umma_f8(d_tmem, w_d + 2 * k, a_d + 2 * k, idesc, accumulate);
+            else umma_bf16(d_tmem, w_d + 2 * k, a_d + 2 * k, idesc, accumulate);
           }
           umma_commit(bar_empty + 8 * s);
-          if (++s == kStages) { s = 0; ph ^= 1; }
+          if (kb + 1 == end) umma_commit(bar_tfull + 8 * acc);
         }
-        if (!ok) break;
-        umma_commit(bar_tfull + 8 * acc);
-        if (kChunked && ++acc == 2) { acc = 0; acc_ph ^= 1; }
+        __syncwarp();
+        if (++s == kStages) { s = 0; ph ^= 1; }
       }
+      if (kChunked && ++acc == 2) { acc = 0; acc_ph ^= 1; }
     }
   } else {
     const int ew = warp - 2, quarter = warp & 3;
     const int col0 = (ew >> 2) * C::kColsPerWarp;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + col0;
     const int chunks = kChunked ? (kb_end - kb_begin + kChunkKb - 1) / kChunkKb : 1;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t n = n0 + (vec ? 4 * lane + k : lane + 32 * k);
+      sw[k] = n < p.N ? w_scale_at(p, n) : 0.f;
+      bs[k] = n < p.N ? bias_at(p, n) : 0.f;
+    }
     float sum[C::kColsPerWarp] = {};
     int acc = 0;
     uint32_t acc_ph = 0;
     bool ok = true;
     for (int ch = 0; ch < chunks; ++ch) {
-      if (!(ok = mbar_wait(bar_tfull + 8 * acc, acc_ph, abort_flag, p.status, 8u))) break;
+      if (!(ok = mbar_wait_warp(bar_tfull + 8 * acc, acc_ph, abort_flag, p.status, 8u))) break;
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < C::kColsPerWarp; c += 16) {
@@ -575,23 +733,9 @@ scaled_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   tc_fence_before();
   cluster_sync_all();  // every CTA's partial sums are in place
   if (warp >= 2) {
-    const int64_t n = (int64_t)n_t * 128 + (warp & 3) * 32 + lane;
-    const int64_t m0 = (int64_t)m_t * NT;
     const int rows = (int)min((int64_t)NT, p.M - m0);
-    const uint32_t partial = smem_base + ((warp & 3) * 32 + lane) * 4;
-    const int first = (warp - 2) >> 2;
-    constexpr int step = C::kWarpsPerQuarter;
-    if (n < p.N) {
-      switch (p.activation) {
-        case B200_ACT_RELU: finish_split_t<OUT, B200_ACT_RELU>(p, partial, ranks, rank, first, step, m0, rows, n); break;
-        case B200_ACT_GELU: finish_split_t<OUT, B200_ACT_GELU>(p, partial, ranks, rank, first, step, m0, rows, n); break;
-        case B200_ACT_GELU_TANH:
-          finish_split_t<OUT, B200_ACT_GELU_TANH>(p, partial, ranks, rank, first, step, m0, rows, n);
-          break;
-        case B200_ACT_SILU: finish_split_t<OUT, B200_ACT_SILU>(p, partial, ranks, rank, first, step, m0, rows, n); break;
-        default: finish_split_t<OUT, B200_ACT_NONE>(p, partial, ranks, rank, first, step, m0, rows, n);
-      }
-    }
+    if (vec) finish_split<OUT, true>(p, smem_base, ranks, rank, warp - 2, C::kEpilogueWarps, lane, m0, rows, n0, sw, bs);
+    else finish_split<OUT, false>(p, smem_base, ranks, rank, warp - 2, C::kEpilogueWarps, lane, m0, rows, n0, sw, bs);
   }
   __syncwarp();
   cluster_sync_all();  // no CTA leaves while another reads its partial sums
@@ -625,7 +769,7 @@ struct Plan {
 struct Operands {
   const void *A, *W;
   int64_t K, a_pitch, w_pitch;
-  int type;
+  int type, y_type;
 };
 
 template <bool F8, typename OUT, int BN>
@@ -655,14 +799,17 @@ int launch_pair(cudaStream_t st, const Operands &o, ScaledParams &p) {
       return fail(B200_ECUDA, "gemm_scaled: cudaOccupancyMaxActiveClusters failed");
     max_pairs[dev].store(n, std::memory_order_relaxed);
   }
-  CUtensorMap ma, mw;
-  if (int rc = encode_map_rows(&ma, o.A, o.type, o.K, p.M, o.a_pitch, 128)) return rc;
-  if (int rc = encode_map_rows(&mw, o.W, o.type, o.K, p.N, o.w_pitch, BN / 2)) return rc;
+  CUtensorMap ma, mw, my;
+  if (int rc = encode_map_2d(&ma, o.A, o.type, o.K, p.M, o.a_pitch, F8 ? 128 : 64, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  if (int rc = encode_map_2d(&mw, o.W, o.type, o.K, p.N, o.w_pitch, F8 ? 128 : 64, BN / 2, CU_TENSOR_MAP_SWIZZLE_128B))
+    return rc;
+  const int64_t y_pitch = p.M > 1 ? p.ldy * (int64_t)sizeof(OUT) : (p.N * (int64_t)sizeof(OUT) + 15) / 16 * 16;
+  if (int rc = encode_map_2d(&my, p.Y, o.y_type, p.N, p.M, y_pitch, kBlockCols<OUT>, 32, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
   p.num_m_tiles = (int)((p.M + 255) / 256);
   p.num_n_tiles = (int)((p.N + BN - 1) / BN);
   p.idesc |= (uint32_t)(BN >> 3) << 17 | (uint32_t)(256 >> 4) << 24;
   const int64_t tiles = (int64_t)p.num_m_tiles * p.num_n_tiles, cap = max_pairs[dev].load(std::memory_order_relaxed);
-  kern<<<(unsigned)(2 * (tiles < cap ? tiles : cap)), C::kThreads, C::kSmemBytes, st>>>(ma, mw, p);
+  kern<<<(unsigned)(2 * (tiles < cap ? tiles : cap)), C::kThreads, C::kSmemBytes, st>>>(ma, mw, my, p);
   return check_launch("gemm_scaled(pair)");
 }
 
@@ -673,8 +820,8 @@ int launch_split(cudaStream_t st, const Operands &o, ScaledParams &p, int ranks)
   static std::atomic<uint64_t> smem_set{0};
   if (int rc = raise_smem(kern, C::kSmemBytes, smem_set)) return rc;
   CUtensorMap ma, mw;
-  if (int rc = encode_map_rows(&ma, o.A, o.type, o.K, p.M, o.a_pitch, NT)) return rc;
-  if (int rc = encode_map_rows(&mw, o.W, o.type, o.K, p.N, o.w_pitch, 128)) return rc;
+  if (int rc = encode_map_2d(&ma, o.A, o.type, o.K, p.M, o.a_pitch, F8 ? 128 : 64, NT, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  if (int rc = encode_map_2d(&mw, o.W, o.type, o.K, p.N, o.w_pitch, F8 ? 128 : 64, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   p.num_m_tiles = (int)((p.M + NT - 1) / NT);
   p.num_n_tiles = (int)((p.N + 127) / 128);
   p.idesc |= (uint32_t)(NT >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
@@ -742,7 +889,7 @@ int run_plan(cudaStream_t st, const b200_gemm_scaled_desc &d, const Plan &plan, 
   p.Y = Y;
   p.status = device_status_ptr();
   if (!p.status) return fail(B200_ECUDA, "gemm_scaled: device status word unavailable");
-  const Operands o = {A, W, d.K, d.lda * b, d.ldw * b, d.type};
+  const Operands o = {A, W, d.K, d.lda * b, d.ldw * b, d.type, d.y_type};
   const bool f8 = d.type == B200_TYPE_E4M3;
   switch (d.y_type) {
     case B200_TYPE_F32: return f8 ? launch_plan<true, float>(st, o, p, plan) : launch_plan<false, float>(st, o, p, plan);
@@ -752,10 +899,10 @@ int run_plan(cudaStream_t st, const b200_gemm_scaled_desc &d, const Plan &plan, 
   }
 }
 
-// Widest access with which every row of `q` can be read or written: 32, 16 or fewer (0) bytes.
+// Widest access with which every row of `q` can be read or written: 32, 16, 8 or fewer (0) bytes.
 int row_access(const void *q, int64_t rows, int64_t ld, int bytes) {
   const uint64_t bits = reinterpret_cast<uintptr_t>(q) | (rows > 1 ? (uint64_t)(ld * bytes) : 0);
-  return bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : 0;
+  return bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : 0;
 }
 
 bool is_float(int type) { return type == B200_TYPE_F32 || type == B200_TYPE_F16 || type == B200_TYPE_BF16; }

@@ -1332,23 +1332,23 @@ int tc::encode_map_bf16(CUtensorMap *map, const void *base, uint64_t k, uint64_t
   return B200_OK;
 }
 
-int tc::encode_map_rows(CUtensorMap *map, const void *base, int type, uint64_t k, uint64_t rows, uint64_t pitch_bytes,
-                        uint32_t box_rows) {
+int tc::encode_map_2d(CUtensorMap *map, const void *base, int type, uint64_t cols, uint64_t rows, uint64_t pitch_bytes,
+                      uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return fail(B200_ECUDA, "cuTensorMapEncodeTiled entry point not available");
-  const bool f8 = type == B200_TYPE_E4M3;
-  cuuint64_t gdim[2] = {k, rows};
+  const CUtensorMapDataType element = type == B200_TYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                      : type == B200_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                      : type == B200_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                               : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  cuuint64_t gdim[2] = {cols, rows};
   cuuint64_t gstr[1] = {pitch_bytes};
-  cuuint32_t box[2] = {f8 ? 128u : 64u, box_rows};
+  cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map,
-                  f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                     : type == B200_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                  2, const_cast<void *>(base), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = fn(map, element, 2, const_cast<void *>(base), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
-    return fail(B200_ECUDA, "cuTensorMapEncodeTiled (rows) failed (%d): k %llu rows %llu pitch %llu box rows %u", (int)r,
-                (unsigned long long)k, (unsigned long long)rows, (unsigned long long)pitch_bytes, box_rows);
+    return fail(B200_ECUDA, "cuTensorMapEncodeTiled (2d) failed (%d): %llu x %llu, pitch %llu, box %u x %u", (int)r,
+                (unsigned long long)cols, (unsigned long long)rows, (unsigned long long)pitch_bytes, box_cols, box_rows);
   return B200_OK;
 }
 

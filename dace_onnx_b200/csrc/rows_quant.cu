@@ -17,7 +17,7 @@ namespace b200 {
 namespace {
 
 constexpr int kRowsPerCta = 8;         // rows of a CTA of the warp-per-row form
-constexpr int kMaxBlock = 512;          // of a row held in registers: 32 values a thread of both inputs need ~100 registers
+constexpr int kMaxBlock = 1024;
 constexpr int kLongBlock = 1024;
 
 struct RowParams {
@@ -32,26 +32,32 @@ struct RowParams {
   bool gamma_f32;  // gamma is fp32 although x is not
 };
 
-// VEC adjacent values: one 16-byte access (VEC * sizeof(T) == 16), or one value.
+// VEC adjacent values: one 16-byte access (VEC * sizeof(T) == 16), or one value. They are kept as loaded until they are
+// used: two inputs of 16 bits then take no more registers than one row of fp32.
 template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T *p, float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    v[0] = to_f32<T>(*p);
-  } else {
-    uint4 u;
+struct Raw {
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const T *p) {
     // plain (not .nc): an output may be the same rows, written later by the thread that read them
     asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                  : "l"(p)
                  : "memory");
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  }
+  __device__ __forceinline__ void get(float (&v)[VEC]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
       else unpack2<T>(w[i], v[2 * i], v[2 * i + 1]);
     }
   }
-}
+};
+template <typename T>
+struct Raw<T, 1> {
+  T w;
+  __device__ __forceinline__ void load(const T *p) { w = *p; }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = to_f32<T>(w); }
+};
 template <typename T, int VEC>
 __device__ __forceinline__ void store_vec(T *p, const float (&v)[VEC]) {
   if constexpr (VEC == 1) {
@@ -112,8 +118,12 @@ __device__ __forceinline__ float activate(int act, float x) {
 }
 template <int ACT, int VEC>
 __device__ __forceinline__ void gate_vec(float (&v)[VEC], const float (&z)[VEC]) {
+  if constexpr (VEC == 1) {
+    v[0] *= activate_t<ACT>(z[0]);
+  } else {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) v[i] *= activate_t<ACT>(z[i]);
+    for (int i = 0; i < VEC; i += 2) (Pair(v[i], v[i + 1]) * activate2_t<ACT>(Pair(z[i], z[i + 1]))).get(v[i], v[i + 1]);
+  }
 }
 
 __device__ __forceinline__ uint32_t warp_umax(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
@@ -139,9 +149,12 @@ __device__ __forceinline__ void join(float &sum, uint32_t &top, float *red) {
 // `top` is the pattern of max|y|: the floor keeps 448 / max finite; a NaN fails the comparison and stays.
 __device__ __forceinline__ float row_max(float top) { return top < kTinyRowMax ? kTinyRowMax : top; }
 
+// Threads of a CTA that holds a row: the registers of 8 values allow two CTAs of 1024 threads on an SM, of more one.
+constexpr int row_ctas(int values) { return values <= 8 ? 2 : 1; }
+
 // The row in registers, NV accesses of VEC values a thread. NORM: z is the residual; otherwise z is the gate.
 template <typename T, bool NORM, bool CODES, int VEC, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? kRowsPerCta * 32 : kMaxBlock, WARP ? 2 : 1)
+__global__ void __launch_bounds__(WARP ? kRowsPerCta * 32 : kMaxBlock, WARP ? 2 : row_ctas(VEC * NV))
 rows_kernel(const RowParams p) {
   __shared__ float red[64];
   const int lanes = WARP ? 32 : blockDim.x;
@@ -150,66 +163,54 @@ rows_kernel(const RowParams p) {
   if (WARP && row >= p.rows) return;
   const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
   const T *z = static_cast<const T *>(p.z) + (p.z ? row * p.z_stride : 0);
+  T *h = static_cast<T *>(p.h) + (p.h ? row * p.h_stride : 0);
+  Raw<T, VEC> xr[NV], zr[NV];
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int c = (n * lanes + t) * VEC;
+    if (c < p.len) {
+      xr[n].load(x + c);
+      if (p.z) zr[n].load(z + c);
+    }
+  }
   float v[NV][VEC];
   float sum = 0.f;
   uint32_t top = 0;
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
     const int c = (n * lanes + t) * VEC;
-    if (c < p.len) load_vec<T, VEC>(x + c, v[n]);
-  }
-  if (p.z) {
-    float w[NV][VEC];
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int c = (n * lanes + t) * VEC;
-      if (c < p.len) load_vec<T, VEC>(z + c, w[n]);
-    }
-    if (NORM) {
-      T *h = static_cast<T *>(p.h) + row * p.h_stride;
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const int c = (n * lanes + t) * VEC;
-        if (c < p.len) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) v[n][i] += w[n][i];
-          store_vec<T, VEC>(h + c, v[n]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const int c = (n * lanes + t) * VEC;
-        if (c < p.len) {
-          switch (p.activation) {  // uniform
-            case B200_ACT_RELU: gate_vec<B200_ACT_RELU, VEC>(v[n], w[n]); break;
-            case B200_ACT_GELU: gate_vec<B200_ACT_GELU, VEC>(v[n], w[n]); break;
-            case B200_ACT_GELU_TANH: gate_vec<B200_ACT_GELU_TANH, VEC>(v[n], w[n]); break;
-            case B200_ACT_SILU: gate_vec<B200_ACT_SILU, VEC>(v[n], w[n]); break;
-            default: gate_vec<B200_ACT_NONE, VEC>(v[n], w[n]);
-          }
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int n = 0; n < NV; ++n) {
-    const int c = (n * lanes + t) * VEC;
-    if (c < p.len) {
+    if (c >= p.len) continue;
+    xr[n].get(v[n]);
+    if (p.z) {
+      float w[VEC];
+      zr[n].get(w);
       if (NORM) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sum = fmaf(v[n][i], v[n][i], sum);
-        if (p.gamma) {
-          float g[VEC];
-          load_gamma<T, VEC>(p, c, g);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) v[n][i] *= g[i];
+        for (int i = 0; i < VEC; ++i) v[n][i] += w[i];
+        store_vec<T, VEC>(h + c, v[n]);
+      } else {
+        switch (p.activation) {  // uniform
+          case B200_ACT_RELU: gate_vec<B200_ACT_RELU, VEC>(v[n], w); break;
+          case B200_ACT_GELU: gate_vec<B200_ACT_GELU, VEC>(v[n], w); break;
+          case B200_ACT_GELU_TANH: gate_vec<B200_ACT_GELU_TANH, VEC>(v[n], w); break;
+          case B200_ACT_SILU: gate_vec<B200_ACT_SILU, VEC>(v[n], w); break;
+          default: gate_vec<B200_ACT_NONE, VEC>(v[n], w);
         }
       }
-      if (CODES) {
+    }
+    if (NORM) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(v[n][i]) & 0x7fffffffu);
+      for (int i = 0; i < VEC; ++i) sum = fmaf(v[n][i], v[n][i], sum);
+      if (p.gamma) {
+        float g[VEC];
+        load_gamma<T, VEC>(p, c, g);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[n][i] *= g[i];
       }
+    }
+    if (CODES) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(v[n][i]) & 0x7fffffffu);
     }
   }
   join<WARP>(sum, top, red);
@@ -292,16 +293,19 @@ int dispatch(cudaStream_t st, const RowParams &p, bool vec) {
   constexpr int V = 16 / (int)sizeof(T);
   const int per = vec ? V : 1;                     // values of one access
   const int units = (p.len + per - 1) / per;       // accesses of a row (len is a multiple of V when vec)
-  // Values a thread holds at most: 32, or 16 where each needs an address and a bounds check of its own.
-  const int most = vec ? 32 : 16;
-  // A warp takes a row that fits into its registers; a longer one takes a CTA with about 16 values a thread.
-  const bool warp = units <= 32 * (most / per);
-  int nv = 1;
+  // Accesses of a thread, measured at 6.1 to 6.5 TB/s: two (four with a gate, whose arithmetic hides behind more
+  // loads), and more where the CTA would have over 512 threads (8192 x 8192 bf16 norm: 1024 threads 84 us, 512 threads
+  // 73 us; 8192 x 14336 gate: 896 threads 149 us, 448 threads 107 us). Few rows leave SMs idle: one access each, for
+  // the shortest way through a row. A warp takes a row that four accesses of it hold.
+  const bool few = p.rows <= 2 * kNumSMs;
+  const int most = vec ? 32 / V : 16;
+  const bool warp = units <= 128 && (!vec || p.rows >= kRowsPerCta * kNumSMs);
+  int nv = warp ? 1 : few ? 1 : NORM || !p.z ? 2 : 4;
   if (warp) {
     while (nv * 32 < units) nv *= 2;
   } else {
-    nv = 16 / per;
-    while (nv * kMaxBlock < units && nv * per < most) nv *= 2;
+    if (!vec) nv = 4;
+    while (nv < most && nv * (few || !vec ? kMaxBlock : 512) < units) nv *= vec ? 2 : 4;
     if (nv * kMaxBlock < units) {
       long_rows_kernel<T, NORM, CODES><<<(unsigned)p.rows, kLongBlock, 0, st>>>(p);
       return check_launch("rows(long)");

@@ -85,6 +85,19 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map
       : "memory");
 }
 
+// Store of a box from shared memory, clipped at the tensor's edges; completion by the issuing thread's bulk groups.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
+               ::"l"(map), "r"(src), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// every store of this thread has read its shared memory / is complete
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// this thread's shared-memory writes become visible to bulk copies
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 __device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(ncols) : "memory");
 }
@@ -353,10 +366,10 @@ int encode_map(CUtensorMap *map, const float *base, const uint64_t dims[4], cons
 // rank-2 bf16 tensor map (K-major matrix: dims {K, rows}, row pitch in bytes), 128-byte swizzle
 int encode_map_bf16(CUtensorMap *map, const void *base, uint64_t k, uint64_t rows, uint64_t pitch_bytes, uint32_t box_k,
                     uint32_t box_rows);
-// rank-2 map of a K-major matrix of 1- or 2-byte elements (type: a B200_TYPE_* code), boxes of 128 bytes x box_rows,
-// 128-byte swizzle, zeros past the edges
-int encode_map_rows(CUtensorMap *map, const void *base, int type, uint64_t k, uint64_t rows, uint64_t pitch_bytes,
-                    uint32_t box_rows);
+// rank-2 map of a matrix of elements of `type` (a B200_TYPE_* code), rows pitch_bytes apart: boxes of box_cols x box_rows,
+// zeros past the edges (loads) or nothing written there (stores)
+int encode_map_2d(CUtensorMap *map, const void *base, int type, uint64_t cols, uint64_t rows, uint64_t pitch_bytes,
+                  uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle);
 // rank-5 fp32 tensor map with an explicit box
 int encode_map5(CUtensorMap *map, const float *base, const uint64_t dims[5], const uint64_t strides_bytes[4],
                 const uint32_t box[5], CUtensorMapSwizzle swizzle);
