@@ -19,20 +19,28 @@ OPERAND_TYPES = {E4M3: TYPE_E4M3, torch.float16: TYPE_F16, torch.bfloat16: TYPE_
 
 
 def _act(activation):
-    code = ACTIVATIONS.get("none" if activation is None else activation)
+    code = ACTIVATIONS.get(activation)
     if code is None:
+        if activation is None:
+            return 0
         raise ValueError("activation must be one of %s or None" % sorted(ACTIVATIONS))
     return code
 
 
-def _tensor(t, name, like=None):
+def _device(t, name):
+    """Index of the CUDA device of a tensor."""
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a torch.Tensor" % name)
-    if not t.is_cuda:
+    device = t.get_device()
+    if device < 0:
         raise ValueError("%s must live on a CUDA device (this library has no CPU path)" % name)
-    if like is not None and t.get_device() != like.get_device():
+    return device
+
+
+def _on(device, t, name):
+    if not isinstance(t, torch.Tensor) or t.get_device() != device:
+        _device(t, name)
         raise ValueError("%s must be on the same device as the first operand" % name)
-    return t
 
 
 def _float_type(t, name):
@@ -44,14 +52,15 @@ def _float_type(t, name):
 
 def _row_stride(t):
     """Elements from one row (last axis) to the next, or None when the rows are not evenly spaced or not adjacent."""
-    shape, stride = t.shape, t.stride()
+    shape = t.shape
+    if t.is_contiguous():
+        return shape[-1]
+    stride = t.stride()
     n = len(shape)
     if stride[-1] != 1 and shape[-1] != 1:
         return None
     if n == 2:
         return stride[0] if shape[0] > 1 else shape[1]
-    if t.numel() == 0:
-        return shape[-1]
     step = None  # spacing of the merged leading axes, from the innermost that is not 1
     extent = 1
     for i in range(n - 2, -1, -1):
@@ -68,6 +77,8 @@ def _row_stride(t):
 
 def _input_rows(t):
     """(tensor, row stride): the tensor itself where its rows are evenly spaced, a contiguous copy elsewhere."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
     s = _row_stride(t)
     if s is None:
         t = t.contiguous()
@@ -75,36 +86,38 @@ def _input_rows(t):
     return t, s
 
 
-def _output_rows(t, name, shape, dtype, like):
-    _tensor(t, name, like)
-    if t.dtype != dtype:
+def _output_rows(t, name, shape, dtype, device):
+    """Row stride of an output. shape: a tuple."""
+    _on(device, t, name)
+    if t.dtype is not dtype:
         raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
     if t.shape != shape:
         raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    if t.is_contiguous():
+        return shape[-1]
     s = _row_stride(t)
     if s is None or (s < shape[-1] and t.numel() > shape[-1]):
         raise ValueError("%s: the rows of an output must be evenly spaced, without overlap, their elements adjacent" % name)
     return s
 
 
-def _scales(t, shape, like):
-    if t is None:
-        return torch.empty(shape, device=like.device, dtype=torch.float32)
-    _tensor(t, "scale", like)
-    if t.dtype != torch.float32:
+def _scales(t, shape, device):
+    _on(device, t, "scale")
+    if t.dtype is not torch.float32:
         raise TypeError("scale must be float32, got %s" % t.dtype)
     if t.shape != shape or not t.is_contiguous():
         raise ValueError("scale must be contiguous with shape %s" % (tuple(shape),))
-    return t
 
 
 def _call(fn, device, *args):
     """Launch on the current stream of `device`, which need not be the current device."""
     if device == torch._C._cuda_getDevice():
-        check(fn(torch._C._cuda_getCurrentRawStream(device), *args))
+        status = fn(torch._C._cuda_getCurrentRawStream(device), *args)
     else:
         with torch.cuda.device(device):
-            check(fn(torch._C._cuda_getCurrentRawStream(device), *args))
+            status = fn(torch._C._cuda_getCurrentRawStream(device), *args)
+    if status:
+        check(status)
 
 
 def empty_codes(shape, device):
@@ -116,41 +129,54 @@ def empty_codes(shape, device):
 
 
 def _rmsnorm(x, gamma, residual, eps, out, scale, residual_out, codes):
-    _tensor(x, "x")
-    code = _float_type(x, "x")
+    device = _device(x, "x")
+    dtype = x.dtype
+    code = FLOAT_TYPES.get(dtype)
+    if code is None:
+        code = _float_type(x, "x")
     shape = x.shape
     if len(shape) == 0 or shape[-1] == 0:
         raise ValueError("rmsnorm: rows need at least one value")
     length = shape[-1]
-    rows = x.numel() // length
     xr, xs = _input_rows(x)
-    rr, rs, hs = None, 0, 0
+    rp, hp, rs, hs = None, None, 0, 0
     if residual is not None:
-        _tensor(residual, "residual", x)
-        if residual.dtype != x.dtype or residual.shape != shape:
+        _on(device, residual, "residual")
+        if residual.dtype is not dtype or residual.shape != shape:
             raise ValueError("rmsnorm: residual must have the shape and type of x")
         rr, rs = _input_rows(residual)
         if residual_out is None:
-            residual_out = torch.empty(shape, device=x.device, dtype=x.dtype)
-        hs = _output_rows(residual_out, "residual_out", shape, x.dtype, x)
+            residual_out = torch.empty(shape, device=x.device, dtype=dtype)
+        hs = _output_rows(residual_out, "residual_out", shape, dtype, device)
+        rp, hp = rr.data_ptr(), residual_out.data_ptr()
     elif residual_out is not None:
         raise ValueError("rmsnorm: residual_out needs a residual")
-    gtype = code
+    gp, gtype = None, code
     if gamma is not None:
-        _tensor(gamma, "gamma", x)
-        if gamma.dtype not in (x.dtype, torch.float32) or gamma.numel() != length or gamma.dim() != 1:
-            raise ValueError("rmsnorm: gamma must be [%d], of the type of x or float32" % length)
-        gamma = gamma.contiguous()
-        gtype = FLOAT_TYPES[gamma.dtype]
+        _on(device, gamma, "gamma")
+        if gamma.dtype is not dtype:
+            if gamma.dtype is not torch.float32:
+                raise ValueError("rmsnorm: gamma must be of the type of x or float32")
+            gtype = TYPE_F32
+        if gamma.dim() != 1 or gamma.shape[0] != length:
+            raise ValueError("rmsnorm: gamma must be [%d]" % length)
+        if not gamma.is_contiguous():
+            gamma = gamma.contiguous()
+        gp = gamma.data_ptr()
+    ytype, ydtype = (TYPE_E4M3, E4M3) if codes else (code, dtype)
     if out is None:
-        out = empty_codes(shape, x.device) if codes else torch.empty(shape, device=x.device, dtype=x.dtype)
-    ys = _output_rows(out, "out", shape, E4M3 if codes else x.dtype, x)
+        out = empty_codes(shape, x.device) if codes else torch.empty(shape, device=x.device, dtype=dtype)
+    ys = _output_rows(out, "out", shape, ydtype, device)
+    sp = None
     if codes:
-        scale = _scales(scale, shape[:-1], x)
-    d = RmsnormDesc(rows, length, xs, rs, hs, ys, code, gtype, TYPE_E4M3 if codes else code, float(eps))
-    _call(_lib.load().b200_rmsnorm, x.get_device(), ctypes.byref(d), xr.data_ptr(),
-          None if rr is None else rr.data_ptr(), None if gamma is None else gamma.data_ptr(),
-          None if rr is None else residual_out.data_ptr(), out.data_ptr(), scale.data_ptr() if codes else None)
+        if scale is None:
+            scale = torch.empty(shape[:-1], device=x.device, dtype=torch.float32)
+        else:
+            _scales(scale, shape[:-1], device)
+        sp = scale.data_ptr()
+    rows = shape[0] if len(shape) == 2 else x.numel() // length
+    d = RmsnormDesc(rows, length, xs, rs, hs, ys, code, gtype, ytype, eps)
+    _call(_lib.load().b200_rmsnorm, device, ctypes.byref(d), xr.data_ptr(), rp, gp, hp, out.data_ptr(), sp)
     return out, scale, residual_out
 
 
@@ -177,39 +203,42 @@ def quantize_rows(x, *, gate=None, activation=None, out=None, scale=None):
 
     activation: None / "none", "relu", "gelu", "gelu_tanh" or "silu"; it belongs to the gate. x and gate may be halves of one
     tensor (rows further apart than they are long)."""
-    _tensor(x, "x")
+    device = _device(x, "x")
     code = _float_type(x, "x")
     shape = x.shape
     if len(shape) == 0 or shape[-1] == 0:
         raise ValueError("quantize_rows: rows need at least one value")
     act = _act(activation)
     length = shape[-1]
-    rows = x.numel() // length
     xr, xs = _input_rows(x)
-    gr, gs = None, 0
+    gp, gs = None, 0
     if gate is not None:
-        _tensor(gate, "gate", x)
+        _on(device, gate, "gate")
         if gate.dtype != x.dtype or gate.shape != shape:
             raise ValueError("quantize_rows: gate must have the shape and type of x")
         gr, gs = _input_rows(gate)
+        gp = gr.data_ptr()
     elif act:
         raise ValueError("quantize_rows: an activation belongs to a gate")
     if out is None:
         out = empty_codes(shape, x.device)
-    qs = _output_rows(out, "out", shape, E4M3, x)
-    scale = _scales(scale, shape[:-1], x)
+    qs = _output_rows(out, "out", shape, E4M3, device)
+    if scale is None:
+        scale = torch.empty(shape[:-1], device=x.device, dtype=torch.float32)
+    else:
+        _scales(scale, shape[:-1], device)
+    rows = shape[0] if len(shape) == 2 else x.numel() // length
     d = QuantizeDesc(rows, length, xs, gs, qs, code, act)
-    _call(_lib.load().b200_quantize_rows, x.get_device(), ctypes.byref(d), xr.data_ptr(),
-          None if gr is None else gr.data_ptr(), out.data_ptr(), scale.data_ptr())
+    _call(_lib.load().b200_quantize_rows, device, ctypes.byref(d), xr.data_ptr(), gp, out.data_ptr(), scale.data_ptr())
     return out, scale
 
 
-def _operand(t, name, code, like):
-    """(tensor, row stride) as the product reads it: 16-byte aligned rows; a copy in that layout for any other."""
-    s = _row_stride(t)
-    size = 1 if code == TYPE_E4M3 else 2
-    if s is None or t.data_ptr() % 16 or ((s * size) % 16 and t.numel() > t.shape[-1]) or (s == 0 and t.numel() > t.shape[-1]):
-        k = t.shape[-1]
+def _operand(t, size):
+    """(tensor, row stride) as the product reads it: rows that start at multiples of 16 bytes; any other is copied into such
+    rows. size: bytes of an element."""
+    k = t.shape[-1]
+    s = k if t.is_contiguous() else _row_stride(t)
+    if s is None or t.data_ptr() % 16 or ((s * size % 16 or s < k) and t.numel() > k):
         pitch = -(-k * size // 16) * 16 // size
         padded = torch.empty(t.shape[:-1] + (pitch,), device=t.device, dtype=t.dtype)[..., :k]
         padded.copy_(t)
@@ -217,18 +246,17 @@ def _operand(t, name, code, like):
     return t, s
 
 
-def _scale_operand(t, name, rows, like):
-    """(tensor, step) of a scale operand: one entry, or one a row."""
-    if t is None:
-        return None, 0
-    _tensor(t, name, like)
-    if t.dtype != torch.float32:
+def _scale_operand(t, name, rows, device):
+    """(tensor, step) of a scale operand: one entry for all rows, or one a row."""
+    _on(device, t, name)
+    if t.dtype is not torch.float32:
         raise TypeError("%s must be float32, got %s" % (name, t.dtype))
-    if t.numel() == 1:
-        return t, 0
-    if t.numel() != rows:
+    n = t.numel()
+    if n == rows:
+        return t if t.is_contiguous() else t.contiguous(), 1
+    if n != 1:
         raise ValueError("%s must have one entry, or one for each of the %d rows" % (name, rows))
-    return t.contiguous(), 1
+    return t, 0
 
 
 def matmul_scaled(A, W, *, a_scale=None, w_scale=None, bias=None, activation=None, residual=None, out=None, out_dtype=None):
@@ -241,53 +269,68 @@ def matmul_scaled(A, W, *, a_scale=None, w_scale=None, bias=None, activation=Non
 
     Operands whose rows do not start at multiples of 16 bytes are copied into such rows first: keep weights in a
     `PreparedLinear`, codes in tensors from `empty_codes` or the quantisers."""
-    _tensor(A, "A")
-    _tensor(W, "W", A)
+    device = _device(A, "A")
+    _on(device, W, "W")
     code = OPERAND_TYPES.get(A.dtype)
-    if code is None or W.dtype != A.dtype:
+    if code is None or W.dtype is not A.dtype:
         raise TypeError("A and W must both be float8_e4m3fn, float16 or bfloat16, got %s and %s" % (A.dtype, W.dtype))
-    if A.dim() < 1 or W.dim() != 2 or A.shape[-1] != W.shape[1]:
-        raise ValueError("matmul_scaled: A must be [..., K] and W [N, K], got %s and %s" % (tuple(A.shape), tuple(W.shape)))
-    K, N = A.shape[-1], W.shape[0]
+    shape = A.shape
+    if len(shape) < 1 or W.dim() != 2 or shape[-1] != W.shape[1]:
+        raise ValueError("matmul_scaled: A must be [..., K] and W [N, K], got %s and %s" % (tuple(shape), tuple(W.shape)))
+    N, K = W.shape
     if K == 0:
         raise ValueError("matmul_scaled: K must be at least 1")
     act = _act(activation)
-    M = A.numel() // K
-    shape = A.shape[:-1] + (N,)
+    if len(shape) == 2:
+        M = shape[0]
+        shape = (M, N)
+    else:
+        M = A.numel() // K
+        shape = tuple(shape[:-1]) + (N,)
     if out is None:
         dtype = out_dtype if out_dtype is not None else residual.dtype if residual is not None else \
             torch.bfloat16 if code == TYPE_E4M3 else A.dtype
         if dtype not in FLOAT_TYPES:
             raise TypeError("matmul_scaled: the output must be float32, float16 or bfloat16, not %s" % dtype)
         out = torch.empty(shape, device=A.device, dtype=dtype)
-    elif out_dtype is not None and out_dtype != out.dtype:
-        raise TypeError("matmul_scaled: out is %s, not %s" % (out.dtype, out_dtype))
-    ytype = _float_type(out, "out")
-    ldy = _output_rows(out, "out", shape, out.dtype, A)
-    rr, ldr = None, 0
+    else:
+        dtype = out.dtype
+        if out_dtype is not None and out_dtype != dtype:
+            raise TypeError("matmul_scaled: out is %s, not %s" % (dtype, out_dtype))
+    ytype = FLOAT_TYPES.get(dtype)
+    if ytype is None:
+        raise TypeError("out must be float32, float16 or bfloat16, got %s" % dtype)
+    ldy = _output_rows(out, "out", shape, dtype, device)
+    rp, ldr = None, 0
     if residual is not None:
-        _tensor(residual, "residual", A)
-        if residual.dtype != out.dtype or residual.shape != shape:
+        _on(device, residual, "residual")
+        if residual.dtype is not dtype or residual.shape != shape:
             raise ValueError("matmul_scaled: residual must have the output's shape and type")
         rr, ldr = _input_rows(residual)
         if ldr < N and M > 1:
-            rr = residual.contiguous()
-            ldr = N
-    btype = 0
+            rr, ldr = residual.contiguous(), N
+        rp = rr.data_ptr()
+    bp, btype = None, 0
     if bias is not None:
-        _tensor(bias, "bias", A)
+        _on(device, bias, "bias")
         btype = _float_type(bias, "bias")
-        if bias.shape != (N,):
+        if bias.dim() != 1 or bias.shape[0] != N:
             raise ValueError("matmul_scaled: bias must be [%d]" % N)
-        bias = bias.contiguous()
-    a_scale, sa = _scale_operand(a_scale, "a_scale", M, A)
-    w_scale, sw = _scale_operand(w_scale, "w_scale", N, A)
-    A, lda = _operand(A, "A", code, A)
-    W, ldw = _operand(W, "W", code, A)
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
+        bp = bias.data_ptr()
+    sap, sa, swp, sw = None, 0, None, 0
+    if a_scale is not None:
+        a_scale, sa = _scale_operand(a_scale, "a_scale", M, device)
+        sap = a_scale.data_ptr()
+    if w_scale is not None:
+        w_scale, sw = _scale_operand(w_scale, "w_scale", N, device)
+        swp = w_scale.data_ptr()
+    size = 1 if code == TYPE_E4M3 else 2
+    A, lda = _operand(A, size)
+    W, ldw = _operand(W, size)
     d = GemmScaledDesc(M, N, K, lda, ldw, ldy, ldr, sa, sw, code, btype, ytype, act)
-    _call(_lib.load().b200_gemm_scaled, A.get_device(), ctypes.byref(d), A.data_ptr(), W.data_ptr(),
-          None if a_scale is None else a_scale.data_ptr(), None if w_scale is None else w_scale.data_ptr(),
-          None if bias is None else bias.data_ptr(), None if rr is None else rr.data_ptr(), out.data_ptr())
+    _call(_lib.load().b200_gemm_scaled, device, ctypes.byref(d), A.data_ptr(), W.data_ptr(), sap, swp, bp, rp, out.data_ptr())
     return out
 
 
@@ -299,7 +342,7 @@ class PreparedLinear:
     an e4m3 layer, quantise their rows; or e4m3 codes with `a_scale`, as the quantisers return them."""
 
     def __init__(self, weight, bias=None, *, activation=None, dtype=E4M3):
-        _tensor(weight, "weight")
+        device = _device(weight, "weight")
         _float_type(weight, "weight")
         if weight.dim() != 2 or 0 in weight.shape:
             raise ValueError("PreparedLinear: weight must be [N, K]")
@@ -309,7 +352,7 @@ class PreparedLinear:
         self.N, self.K = weight.shape
         self.activation, self.dtype = activation, dtype
         if bias is not None:
-            _tensor(bias, "bias", weight)
+            _on(device, bias, "bias")
             _float_type(bias, "bias")
             if bias.shape != (self.N,):
                 raise ValueError("PreparedLinear: bias must be [%d]" % self.N)
