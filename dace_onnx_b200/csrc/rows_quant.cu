@@ -94,7 +94,7 @@ __device__ __forceinline__ void load_gamma(const RowParams &p, int c, float (&g)
   } else {
     const T *q = static_cast<const T *>(p.gamma) + c;
     if constexpr (VEC == 1) {
-      g[0] = to_f32<T>(*q);
+      g[0] = to_f32<T>(__ldg(q));  // read-only: may be loaded before h is stored
     } else {
       const uint4 u = __ldg(reinterpret_cast<const uint4 *>(q));
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};

@@ -5,12 +5,15 @@ device, nothing synchronised, no CPU path. Tensors are fp32, fp16 or bf16; sums 
 
 8-bit rows are `torch.float8_e4m3fn` codes with one fp32 scale a row, value = code * scale. A new codes tensor has its rows
 start at multiples of 16 bytes (`empty_codes`), the layout in which the product reads them without a copy.
+
+Ordinary calls go through `torch_calls`, which reads the tensors in C++; whatever it declines comes back here, where arguments
+are checked, errors raised and operands in other layouts copied.
 """
 import ctypes
 
 import torch
 
-from . import _lib
+from . import _lib, torch_calls
 from ._lib import ACTIVATIONS, TYPE_BF16, TYPE_E4M3, TYPE_F16, TYPE_F32, GemmScaledDesc, QuantizeDesc, RmsnormDesc, check
 
 FLOAT_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
@@ -129,6 +132,11 @@ def empty_codes(shape, device):
 
 
 def _rmsnorm(x, gamma, residual, eps, out, scale, residual_out, codes):
+    done = torch_calls.rmsnorm(x, gamma, residual, eps, out, scale, residual_out, codes)
+    if done is not None:
+        if type(done) is int:
+            check(done)
+        return done
     device = _device(x, "x")
     dtype = x.dtype
     code = FLOAT_TYPES.get(dtype)
@@ -203,12 +211,17 @@ def quantize_rows(x, *, gate=None, activation=None, out=None, scale=None):
 
     activation: None / "none", "relu", "gelu", "gelu_tanh" or "silu"; it belongs to the gate. x and gate may be halves of one
     tensor (rows further apart than they are long)."""
+    act = _act(activation)
+    done = torch_calls.quantize_rows(x, gate, act, out, scale)
+    if done is not None:
+        if type(done) is int:
+            check(done)
+        return done
     device = _device(x, "x")
     code = _float_type(x, "x")
     shape = x.shape
     if len(shape) == 0 or shape[-1] == 0:
         raise ValueError("quantize_rows: rows need at least one value")
-    act = _act(activation)
     length = shape[-1]
     xr, xs = _input_rows(x)
     gp, gs = None, 0
@@ -269,6 +282,13 @@ def matmul_scaled(A, W, *, a_scale=None, w_scale=None, bias=None, activation=Non
 
     Operands whose rows do not start at multiples of 16 bytes are copied into such rows first: keep weights in a
     `PreparedLinear`, codes in tensors from `empty_codes` or the quantisers."""
+    act = _act(activation)
+    done = torch_calls.matmul_scaled(A, W, a_scale, w_scale, bias, act, residual, out,
+                                     -1 if out_dtype is None else FLOAT_TYPES.get(out_dtype, TYPE_E4M3))
+    if done is not None:
+        if type(done) is int:
+            check(done)
+        return done
     device = _device(A, "A")
     _on(device, W, "W")
     code = OPERAND_TYPES.get(A.dtype)
@@ -280,7 +300,6 @@ def matmul_scaled(A, W, *, a_scale=None, w_scale=None, bias=None, activation=Non
     N, K = W.shape
     if K == 0:
         raise ValueError("matmul_scaled: K must be at least 1")
-    act = _act(activation)
     if len(shape) == 2:
         M = shape[0]
         shape = (M, N)

@@ -71,6 +71,20 @@ def test_products(m, n, k, t, cuda):
         check(y, a, sa, w, sw, bias, "silu", residual)
 
 
+# shapes that between them take every tile and split: 128 and 256 wide pairs, tiles of 16 to 256 rows on 1 to 8 CTAs
+PLANS = [(2371, 64, 68), (4455, 536, 2204), (4154, 515, 66), (4991, 132, 688), (4898, 73, 1535), (1, 64, 904), (10, 64, 2349),
+         (1, 64, 5667), (4993, 401, 3709), (4780, 135, 3993), (4836, 67, 4006), (4739, 70, 64), (1208, 72, 1495), (657, 64, 2915),
+         (4786, 133, 79), (4979, 68, 656), (1189, 64, 3000), (289, 64, 7192), (594, 64, 7511), (593, 136, 7051)]
+
+
+@pytest.mark.parametrize("m,n,k", PLANS)
+def test_every_plan(m, n, k, cuda):
+    a, sa, w, sw = operands(m, n, k, torch.float8_e4m3fn)
+    for out in (torch.bfloat16, torch.float32):
+        bias, residual = make(5, n), make(6, m, n).to(out)
+        check(ops.matmul_scaled(a, w, a_scale=sa, w_scale=sw, bias=bias, residual=residual), a, sa, w, sw, bias, None, residual)
+
+
 @pytest.mark.parametrize("act", [None, "relu", "gelu", "gelu_tanh", "silu"])
 @pytest.mark.parametrize("m,n", [(5, 333), (300, 512)])
 def test_epilogues(m, n, act, cuda):
@@ -180,6 +194,25 @@ def test_prepared_linear(cuda):
                 check(y, x.to(TYPES[t]), None, layer.weight, None, bias, "gelu")
     with pytest.raises(ValueError, match="a_scale"):
         ops.PreparedLinear(weight)(q)
+
+
+def test_checked_path_gives_the_same(cuda, monkeypatch):
+    """Calls that the C++ entry declines take the path that checks and copies in Python: the same bits."""
+    from dace_onnx_b200 import torch_calls
+    for m, n, k in ((5, 100, 333), (300, 264, 512)):
+        a, sa, w, sw = operands(m, n, k, torch.float8_e4m3fn)
+        bias, residual = make(50, n).bfloat16(), make(51, m, n).bfloat16()
+        args = dict(a_scale=sa, w_scale=sw, bias=bias, activation="relu", residual=residual)
+        want = ops.matmul_scaled(a, w, **args)
+        with monkeypatch.context() as p:
+            p.setattr(torch_calls, "matmul_scaled", lambda *_: None)
+            p.setattr(torch_calls, "quantize_rows", lambda *_: None)
+            assert torch.equal(ops.matmul_scaled(a, w, **args), want)
+            out = torch.empty(m, n, device="cuda", dtype=torch.bfloat16)
+            assert ops.matmul_scaled(a, w, out=out, **args) is out and torch.equal(out, want)
+            again = ops.quantize_rows(make(1, m, k))
+            assert torch.equal(again[0].float(), a.float()) and torch.equal(again[1], sa)
+            assert ops.matmul_scaled(a, w, a_scale=sa, w_scale=sw, out_dtype=torch.float32).dtype == torch.float32
 
 
 def test_refusals(cuda):

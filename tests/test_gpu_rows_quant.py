@@ -226,6 +226,25 @@ def test_the_same_call_gives_the_same_bits(cuda):
         assert torch.equal(first[0].view(torch.uint8), again[0].view(torch.uint8)) and torch.equal(first[1], again[1])
 
 
+def test_checked_path_gives_the_same(cuda, monkeypatch):
+    """Calls that the C++ entry declines take the path that checks and copies in Python: the same bits."""
+    from dace_onnx_b200 import torch_calls
+    x, r, g = make(20, 5, 333, t=torch.bfloat16), make(21, 5, 333, t=torch.bfloat16), 1 + make(22, 333, scale=0.1)
+    want = ops.rmsnorm_quantize(x, g, residual=r), ops.rmsnorm(x, g, residual=r), ops.quantize_rows(x, gate=r, activation="gelu")
+    with monkeypatch.context() as p:
+        for name in ("rmsnorm", "quantize_rows"):
+            p.setattr(torch_calls, name, lambda *_: None)
+        got = ops.rmsnorm_quantize(x, g, residual=r), ops.rmsnorm(x, g, residual=r), ops.quantize_rows(x, gate=r, activation="gelu")
+        h, s, q = torch.empty_like(x), torch.empty(5, device="cuda"), ops.empty_codes((5, 333), "cuda")
+        given = ops.rmsnorm_quantize(x, g, residual=r, out=q, scale=s, residual_out=h)
+        assert given[0] is q and given[1] is s and given[2] is h
+    for a, b in zip(want + (want[0],), got + (given,)):
+        for u, v in zip(a, b):
+            assert u.shape == v.shape and u.stride() == v.stride() and torch.equal(u.float(), v.float())
+    given = ops.rmsnorm_quantize(x, g, residual=r, out=q, scale=s, residual_out=h)
+    assert given[0] is q and given[1] is s and given[2] is h
+
+
 def test_refusals(cuda):
     x = make(16, 4, 64)
     with pytest.raises(TypeError):
