@@ -189,6 +189,9 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
     }
   }
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 __device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
 
 __device__ __forceinline__ void teardown_after_abort(int aborted) {
@@ -254,6 +257,9 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   const int64_t num_tiles = (int64_t)p.num_m_tiles * p.num_n_tiles;
 
   if (threadIdx.x == 0) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_w);
+    prefetch_map(&map_y);
     s_abort = 0;
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar_full + 8 * s, 1);   // even CTA: its expect_tx for the bytes of both
@@ -273,6 +279,8 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   __syncthreads();
   cluster_sync_all();
   tc_fence_after();
+  let_next_start();
+  wait_previous();
   const uint32_t tmem_base = s_tmem_base;
   volatile int *abort_flag = &s_abort;
 
@@ -616,6 +624,8 @@ scaled_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   const int kb_begin = (int)((int64_t)p.num_kb * rank / ranks), kb_end = (int)((int64_t)p.num_kb * (rank + 1) / ranks);
 
   if (threadIdx.x == 0) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_w);
     s_abort = 0;
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar_full + 8 * s, 1);
@@ -634,6 +644,8 @@ scaled_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  let_next_start();
+  wait_previous();
   const uint32_t tmem_base = s_tmem_base;
   volatile int *abort_flag = &s_abort;
   const int64_t m0 = (int64_t)m_t * NT, n0 = (int64_t)n_t * 128;
@@ -809,8 +821,8 @@ int launch_pair(cudaStream_t st, const Operands &o, ScaledParams &p) {
   p.num_n_tiles = (int)((p.N + BN - 1) / BN);
   p.idesc |= (uint32_t)(BN >> 3) << 17 | (uint32_t)(256 >> 4) << 24;
   const int64_t tiles = (int64_t)p.num_m_tiles * p.num_n_tiles, cap = max_pairs[dev].load(std::memory_order_relaxed);
-  kern<<<(unsigned)(2 * (tiles < cap ? tiles : cap)), C::kThreads, C::kSmemBytes, st>>>(ma, mw, my, p);
-  return check_launch("gemm_scaled(pair)");
+  return launch_overlapped("gemm_scaled(pair)", kern, (unsigned)(2 * (tiles < cap ? tiles : cap)), C::kThreads, C::kSmemBytes, st, 1,
+                           ma, mw, my, p);
 }
 
 template <bool F8, typename OUT, int NT>
@@ -827,20 +839,8 @@ int launch_split(cudaStream_t st, const Operands &o, ScaledParams &p, int ranks)
   p.idesc |= (uint32_t)(NT >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
   const int64_t ctas = (int64_t)p.num_m_tiles * p.num_n_tiles * ranks;
   if (ctas > 0x7fffffffLL) return fail(B200_EUNSUPPORTED, "gemm_scaled: too many tiles");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
-  cfg.blockDim = dim3(C::kThreads, 1, 1);
-  cfg.dynamicSmemBytes = C::kSmemBytes;
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)ranks;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kern, ma, mw, p, ranks);
-  return check_launch("gemm_scaled(split)");
+  return launch_overlapped("gemm_scaled(split)", kern, (unsigned)ctas, C::kThreads, C::kSmemBytes, st, (unsigned)ranks, ma, mw, p,
+                           ranks);
 }
 
 template <bool F8, typename OUT>

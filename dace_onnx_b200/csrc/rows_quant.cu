@@ -157,6 +157,8 @@ template <typename T, bool NORM, bool CODES, int VEC, int NV, bool WARP>
 __global__ void __launch_bounds__(WARP ? kRowsPerCta * 32 : kMaxBlock, WARP ? 2 : row_ctas(VEC * NV))
 rows_kernel(const RowParams p) {
   __shared__ float red[64];
+  let_next_start();
+  wait_previous();
   const int lanes = WARP ? 32 : blockDim.x;
   const int t = WARP ? (threadIdx.x & 31) : threadIdx.x;
   const int64_t row = WARP ? (int64_t)blockIdx.x * kRowsPerCta + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
@@ -240,6 +242,8 @@ template <typename T, bool NORM, bool CODES>
 __global__ void __launch_bounds__(kLongBlock)
 long_rows_kernel(const RowParams p) {
   __shared__ float red[64];
+  let_next_start();
+  wait_previous();
   const int64_t row = blockIdx.x;
   const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
   const T *z = static_cast<const T *>(p.z) + (p.z ? row * p.z_stride : 0);
@@ -281,11 +285,9 @@ template <typename T, bool NORM, bool CODES, int VEC, int NV>
 int launch_rows(cudaStream_t st, const RowParams &p, bool warp, int threads) {
   if (warp) {
     const int64_t ctas = (p.rows + kRowsPerCta - 1) / kRowsPerCta;
-    rows_kernel<T, NORM, CODES, VEC, NV, true><<<(unsigned)ctas, kRowsPerCta * 32, 0, st>>>(p);
-  } else {
-    rows_kernel<T, NORM, CODES, VEC, NV, false><<<(unsigned)p.rows, threads, 0, st>>>(p);
+    return launch_overlapped("rows", rows_kernel<T, NORM, CODES, VEC, NV, true>, (unsigned)ctas, kRowsPerCta * 32, 0, st, 1, p);
   }
-  return check_launch("rows");
+  return launch_overlapped("rows", rows_kernel<T, NORM, CODES, VEC, NV, false>, (unsigned)p.rows, threads, 0, st, 1, p);
 }
 
 template <typename T, bool NORM, bool CODES>
@@ -307,8 +309,7 @@ int dispatch(cudaStream_t st, const RowParams &p, bool vec) {
     if (!vec) nv = 4;
     while (nv < most && nv * (few || !vec ? kMaxBlock : 512) < units) nv *= vec ? 2 : 4;
     if (nv * kMaxBlock < units) {
-      long_rows_kernel<T, NORM, CODES><<<(unsigned)p.rows, kLongBlock, 0, st>>>(p);
-      return check_launch("rows(long)");
+      return launch_overlapped("rows(long)", long_rows_kernel<T, NORM, CODES>, (unsigned)p.rows, kLongBlock, 0, st, 1, p);
     }
   }
   const int threads = ((units + nv - 1) / nv + 31) / 32 * 32;

@@ -9,6 +9,36 @@
 
 namespace b200 {
 
+// ---- overlapped launches ----------------------------------------------------------------------
+// The kernels of the 8-bit path follow one another in a stream and many last a few microseconds. Each is launched so that it may
+// start while the one before it drains (programmatic stream serialisation): it sets itself up, then waits in wait_previous(),
+// which returns when everything before it in the stream is complete and visible; only after that does it touch
+// global memory. let_next_start() allows the next kernel the same. A kernel with TMEM calls it after its own allocation: a waiting
+// successor could otherwise hold the columns its predecessor still needs.
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename Kernel, typename... Args>
+int launch_overlapped(const char *what, Kernel kern, unsigned grid, unsigned block, size_t smem, cudaStream_t st, unsigned cluster,
+                      const Args &...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kern, args...);
+  return check_launch(what);
+}
+
 constexpr float kE4M3Max = 448.f;
 constexpr float kTinyRowMax = 7.888609052210118e-31f;  // 2^-100: keeps 448 / max finite for rows of zeros
 
