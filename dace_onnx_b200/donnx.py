@@ -84,6 +84,29 @@ def ONNXReduceMean(*, data, reduced, axes, keepdims=1):
     return _out(reduced, lambda o: ops.reduce_mean(data, axes, keepdims, out=o), shape)
 
 
+def ONNXRMSNormalization(*, X, scale, Y, axis=-1, epsilon=1e-5, stash_type=1):
+    """RMSNormalization (ONNX opset 23; not in the reference): over the last axis, computed in fp32. X may be fp16 or bf16 too."""
+    if axis not in (-1, X.dim() - 1):
+        raise NotImplementedError("RMSNormalization: only over the last axis")
+    if stash_type != 1:
+        raise NotImplementedError("RMSNormalization: stash_type must be 1 (float)")
+    return _out(Y, lambda o: ops.rmsnorm(X, scale, eps=epsilon, out=o), X.shape)
+
+
+def ONNXSkipSimplifiedLayerNormalization(*, input, skip, gamma, output, input_skip_bias_sum=None,  # noqa: A002
+                                         epsilon=1e-5):
+    """SkipSimplifiedLayerNormalization (com.microsoft, as exported for decoder models; not in the reference): RMS norm of
+    input + skip; input_skip_bias_sum, when passed, receives that sum."""
+    if input_skip_bias_sum is None:
+        input_skip_bias_sum = torch.empty_like(input, memory_format=torch.contiguous_format)
+
+    def run(total):
+        _out(output, lambda o: ops.rmsnorm(input, gamma, residual=skip, eps=epsilon, out=o, residual_out=total), input.shape)
+
+    _out(input_skip_bias_sum, run, input.shape)
+    return output
+
+
 def _binary(fn, A, B, C):
     shape = torch.broadcast_shapes(A.shape if isinstance(A, torch.Tensor) else (),
                                    B.shape if isinstance(B, torch.Tensor) else ())

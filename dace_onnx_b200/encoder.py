@@ -14,6 +14,10 @@ the contraction epilogues where the graph allows it:
     Reshape/Transpose [0,2,1,3] either side of attention     -> strided batch addressing (no copy)
     ReduceMean..Add (9 nodes)                                -> layernorm
 
+math_mode "fp8" runs the four linear layers on e4m3 operands: weights quantised once with one scale an output, activations
+with one scale a token right before each layer, fp32 accumulation, bias / Gelu / residual in the product's epilogue;
+attention runs in TF32, norms and residuals in fp32.
+
 Torch provides device buffers, streams and (for several GPUs) the process group; all arithmetic
 is in libb200ops.
 """
@@ -55,6 +59,8 @@ class BertEncoderB200:
         self.heads = heads
         self.eps = float(eps)
         self.math_mode = math_mode
+        self.fp8 = math_mode == "fp8"
+        self.attention_mode = "tf32" if self.fp8 else math_mode
         self.micro_batch = int(micro_batch)
         self.fused_attention = bool(fused_attention)
         self.hidden = layers[0]["wq"].shape[0]
@@ -71,6 +77,10 @@ class BertEncoderB200:
                 wo=dev(p["wo"]), bo=dev(p["bo"]), ln1_g=dev(p["ln1_g"]), ln1_b=dev(p["ln1_b"]),
                 wi=dev(p["wi"]), bi=dev(p["bi"]), wo2=dev(p["wo2"]), bo2=dev(p["bo2"]),
                 ln2_g=dev(p["ln2_g"]), ln2_b=dev(p["ln2_b"])))
+            if self.fp8:
+                w = self.layers[-1]
+                for key, bias, act in (("wqkv", "bqkv", None), ("wo", "bo", None), ("wi", "bi", "gelu"), ("wo2", "bo2", None)):
+                    w[key] = ops.PreparedLinear(w[key], w[bias], activation=act)
         self._buf_key = None
         self._buf = None
         self._io = None            # staging buffers and copy streams of forward_host
@@ -85,6 +95,12 @@ class BertEncoderB200:
             e = lambda *s: torch.empty(s, device=self.device, dtype=torch.float32)  # noqa: E731
             self._buf = dict(qkv=e(mb, seq, 3 * h), ctx=e(mb, seq, h), attn=e(mb, seq, h), h1=e(mb, seq, h),
                              inter=e(mb, seq, f), out=e(mb, seq, h), ping=e(mb, seq, h), pong=e(mb, seq, h))
+            if self.fp8:
+                self._buf.update(codes_h=ops.empty_codes((mb * seq, h), self.device),
+                                 codes_f=ops.empty_codes((mb * seq, f), self.device), scale=e(mb * seq),
+                                 # the Gelu's result, which is quantised next: its rounding to 8 bits of mantissa is a
+                                 # sixteenth of e4m3's
+                                 inter=torch.empty((mb, seq, f), device=self.device, dtype=torch.bfloat16))
             self._buf_key = key
         return self._buf
 
@@ -119,23 +135,17 @@ class BertEncoderB200:
 
     # -- one layer on one micro-batch -------------------------------------------------------------
     def _layer(self, x, y, w, buf, b, seq):
-        h, f, nh, d, mm = self.hidden, self.ffn, self.heads, self.head_dim, self.math_mode
+        h, f, mm = self.hidden, self.ffn, self.math_mode
         t = b * seq
         x2 = x.view(t, h)
         qkv, ctx = buf["qkv"][:b], buf["ctx"][:b]
         attn, h1, inter, out = buf["attn"][:b], buf["h1"][:b], buf["inter"][:b], buf["out"][:b]
+        if self.fp8:
+            return self._layer_fp8(x2, y, w, buf, b, seq, qkv, ctx, attn, h1, inter, out)
 
         self._timed("gemm", 2 * t * 3 * h * h, 0, lambda: ops.matmul(
             x2, w["wqkv"], out=qkv.view(t, 3 * h), trans_b=True, epilogue=EPI_BIAS, bias=w["bqkv"], math_mode=mm))
-        # MatMul -> Mul -> Softmax -> MatMul as one kernel when the fused attention covers the case
-        q4 = qkv.view(b, seq, 3 * nh, d)
-        fused = self.fused_attention and self._timed(
-            "attention", 4 * b * nh * seq * seq * d, 16 * t * h,
-            lambda: ops.attention_views(q4[:, :, :nh], q4[:, :, nh:2 * nh], q4[:, :, 2 * nh:], ctx.view(b, seq, nh, d),
-                                        1.0 / math.sqrt(d), math_mode=mm))
-        if fused is False:
-            scores, probs = self._score_buffers(buf["qkv"].shape[0], seq)
-            self._attention_unfused(qkv, scores[:b], probs[:b], ctx, b, seq)
+        self._attention(qkv, ctx, buf, b, seq)
         self._timed("gemm", 2 * t * h * h, 0, lambda: ops.matmul(
             ctx.view(t, h), w["wo"], out=attn.view(t, h), trans_b=True, epilogue=EPI_BIAS_RESIDUAL, bias=w["bo"],
             residual=x2, math_mode=mm))
@@ -149,8 +159,41 @@ class BertEncoderB200:
         self._timed("layernorm", 0, 8 * t * h, lambda: ops.layernorm(out, w["ln2_g"], w["ln2_b"], self.eps, out=y))
         return y
 
+    def _layer_fp8(self, x2, y, w, buf, b, seq, qkv, ctx, attn, h1, inter, out):
+        h, f = self.hidden, self.ffn
+        t = b * seq
+        scale = buf["scale"][:t]
+
+        def linear(key, x, codes, flops, residual, dst):
+            q = codes[:t]
+            self._timed("quantize", 0, x.numel() * (x.element_size() + 1),
+                        lambda: ops.quantize_rows(x, out=q, scale=scale))
+            self._timed("gemm", flops, 0, lambda: w[key](q, a_scale=scale, residual=residual, out=dst))
+
+        linear("wqkv", x2, buf["codes_h"], 2 * t * 3 * h * h, None, qkv.view(t, 3 * h))
+        self._attention(qkv, ctx, buf, b, seq)
+        linear("wo", ctx.view(t, h), buf["codes_h"], 2 * t * h * h, x2, attn.view(t, h))
+        self._timed("layernorm", 0, 8 * t * h, lambda: ops.layernorm(attn, w["ln1_g"], w["ln1_b"], self.eps, out=h1))
+        linear("wi", h1.view(t, h), buf["codes_h"], 2 * t * f * h, None, inter.view(t, f))
+        linear("wo2", inter.view(t, f), buf["codes_f"], 2 * t * f * h, h1.view(t, h), out.view(t, h))
+        self._timed("layernorm", 0, 8 * t * h, lambda: ops.layernorm(out, w["ln2_g"], w["ln2_b"], self.eps, out=y))
+        return y
+
+    def _attention(self, qkv, ctx, buf, b, seq):
+        h, nh, d, mm = self.hidden, self.heads, self.head_dim, self.attention_mode
+        t = b * seq
+        # MatMul -> Mul -> Softmax -> MatMul as one kernel when the fused attention covers the case
+        q4 = qkv.view(b, seq, 3 * nh, d)
+        fused = self.fused_attention and self._timed(
+            "attention", 4 * b * nh * seq * seq * d, 16 * t * h,
+            lambda: ops.attention_views(q4[:, :, :nh], q4[:, :, nh:2 * nh], q4[:, :, 2 * nh:], ctx.view(b, seq, nh, d),
+                                        1.0 / math.sqrt(d), math_mode=mm))
+        if fused is False:
+            scores, probs = self._score_buffers(buf["qkv"].shape[0], seq)
+            self._attention_unfused(qkv, scores[:b], probs[:b], ctx, b, seq)
+
     def _attention_unfused(self, qkv, scores, probs, ctx, b, seq):
-        h, nh, d, mm = self.hidden, self.heads, self.head_dim, self.math_mode
+        h, nh, d, mm = self.hidden, self.heads, self.head_dim, self.attention_mode
         t = b * seq
         # scores[b,n] = q[b,:,n,:] @ k[b,:,n,:]^T * 1/sqrt(d), heads addressed inside qkv
         self._timed("gemm_qk", 2 * b * nh * seq * seq * d, 4 * (2 * t * h + b * nh * seq * seq), lambda: ops.gemm_raw(

@@ -5,7 +5,11 @@ reference's autodiff example (Linear 784->120->32->10), as `@dace_module` would 
 `conv_stack_forward`: [Conv 3x3 pad 1 + bias, Relu] x n -- the README model of the reference
 (tests/pytorch/test_conv2d.py:11-37), NCHW.
 Relu is folded into the producing contraction's epilogue; every node also exists standalone in `ops`.
+`gated_mlp_forward`: RMS norm with the residual's addition, gate and up projections, act(gate) * up, down projection -- the
+feed-forward half of a decoder layer, on 8-bit weights and activations.
 """
+import torch
+
 from . import ops
 
 
@@ -35,3 +39,27 @@ def conv_stack_forward(x, params, math_mode=None, workspace=None):
         h = conv(h, x_nhwc=nhwc, y_nhwc=keep, workspace=workspace)
         nhwc = keep
     return h
+
+
+class GatedMlp:
+    """Set-up of gated_mlp_forward: the weights quantised once to e4m3.
+
+    gamma: [hidden]; w_gate, w_up: [ffn, hidden]; w_down: [hidden, ffn]; CUDA tensors in fp32, fp16 or bf16 (gamma in the
+    activations' type or fp32). activation: what the gate goes through."""
+
+    def __init__(self, gamma, w_gate, w_up, w_down, *, activation="silu", eps=1e-6):
+        if w_gate.dim() != 2 or w_gate.shape != w_up.shape or w_down.shape != w_gate.shape[::-1] or \
+                gamma.shape != w_gate.shape[1:]:
+            raise ValueError("GatedMlp: expected gamma [hidden], w_gate and w_up [ffn, hidden], w_down [hidden, ffn]")
+        self.gamma, self.activation, self.eps, self.ffn = gamma, activation, float(eps), w_gate.shape[0]
+        # one product for both projections: they read the same activations
+        self.gate_up = ops.PreparedLinear(torch.cat([w_gate, w_up]))
+        self.down = ops.PreparedLinear(w_down)
+
+
+def gated_mlp_forward(x, residual, mlp):
+    """(y, h): h = residual + x, y = down(act(gate(n)) * up(n)) with n the RMS norm of h. x, residual: [..., hidden]."""
+    q, s, h = ops.rmsnorm_quantize(x, mlp.gamma, residual=residual, eps=mlp.eps)
+    both = mlp.gate_up(q, a_scale=s, out_dtype=x.dtype)
+    q, s = ops.quantize_rows(both[..., mlp.ffn:], gate=both[..., :mlp.ffn], activation=mlp.activation)
+    return mlp.down(q, a_scale=s, out_dtype=x.dtype), h

@@ -2,7 +2,9 @@
 import pytest
 import torch
 
-from dace_onnx_b200 import ops
+from dace_onnx_b200 import donnx, graphs, ops
+from dace_onnx_b200.encoder import BertEncoderB200
+from oracle import pure_oracle as po
 from tests.test_gpu_rows_quant import make
 
 pytestmark = pytest.mark.gpu
@@ -74,3 +76,66 @@ def test_chain_against_64_bits(cuda):
     both = n @ up.t()
     want = (both[:, :ffn] * torch.sigmoid(both[:, :ffn]) * both[:, ffn:]) @ down.t()
     assert ((y - want).norm() / want.norm()).item() < 0.075
+
+
+def test_gated_mlp_forward(cuda):
+    """The runner makes the calls of the chain above (same bits), on any leading shape; its error as derived there."""
+    hidden, ffn = 520, 776
+    gate, up, down = (make(80 + i, *s, scale=s[1] ** -0.5) for i, s in enumerate([(ffn, hidden), (ffn, hidden), (hidden, ffn)]))
+    gamma = 1 + make(83, hidden, scale=0.1)
+    for act, f in (("silu", torch.nn.functional.silu), ("gelu", torch.nn.functional.gelu)):
+        mlp = graphs.GatedMlp(gamma, gate, up, down, activation=act)
+        for shape in ((3, 7, hidden), (130, hidden)):
+            x, r = make(84, *shape).half(), make(85, *shape).half()
+            y, h = graphs.gated_mlp_forward(x, r, mlp)
+            assert y.shape == h.shape == x.shape and y.dtype == h.dtype == torch.float16
+            h64 = x.double() + r.double()
+            n = h64 / torch.sqrt((h64 * h64).mean(-1, keepdim=True) + 1e-6) * gamma.double()
+            want = (f(n @ gate.double().t()) * (n @ up.double().t())) @ down.double().t()
+            assert ((y.double() - want).norm() / want.norm()).item() < 0.075
+            q, s, h2 = ops.rmsnorm_quantize(x, gamma, residual=r)
+            both = mlp.gate_up(q, a_scale=s, out_dtype=torch.float16)
+            q, s = ops.quantize_rows(both[..., ffn:].contiguous(), gate=both[..., :ffn].contiguous(), activation=act)
+            assert torch.equal(mlp.down(q, a_scale=s, out_dtype=torch.float16), y) and torch.equal(h, h2)
+    with pytest.raises(ValueError, match="expected gamma"):
+        graphs.GatedMlp(gamma, gate, up, down.t())
+
+
+@pytest.mark.parametrize("hidden,heads,ffn,shape", [(256, 4, 1024, (3, 64)), (96, 2, 200, (2, 19))])
+def test_encoder_on_8_bit_weights(hidden, heads, ffn, shape, cuda):
+    """Two layers against the oracle in fp32. Four operands are quantised on the way through each half of a layer, each adding a
+    relative error of at most 2^-3 / sqrt(12) = 0.036 in the 2-norm: 0.072 together, 1.13 times that through the Gelu. The residual
+    is added in fp32, so a half whose branch is at most as large as its stream keeps below 0.072 * 1.13 / sqrt(2) = 0.058, and
+    four halves below 2 * 0.058 (the errors are independent)."""
+    layers = [po.make_bert_layer_params(hidden, ffn, seed=90 + i, std=0.05) for i in range(2)]
+    x = torch.randn(*shape, hidden, generator=torch.Generator().manual_seed(92))
+    ref = po.bert_encoder_forward(x, layers, heads=heads)
+    enc = BertEncoderB200(layers, heads=heads, device=cuda, math_mode="fp8")
+    y = enc.forward_device(x.to(cuda))
+    assert ((y.cpu() - ref).norm() / ref.norm()).item() < 2 * 0.058
+    assert torch.equal(enc(x.pin_memory()), y.cpu())
+    pieces = BertEncoderB200(layers, heads=heads, device=cuda, math_mode="fp8", micro_batch=1)
+    assert ((pieces(x) - ref).norm() / ref.norm()).item() < 2 * 0.058
+
+
+def test_norm_nodes(cuda):
+    x, skip, gamma = make(95, 4, 6, 100), make(96, 4, 6, 100), 1 + make(97, 100, scale=0.1)
+    y = torch.empty_like(x)
+    assert donnx.ONNXRMSNormalization(X=x, scale=gamma, Y=y, epsilon=1e-5) is y
+    assert torch.equal(y, ops.rmsnorm(x, gamma, eps=1e-5))
+    wide = torch.empty(4, 6, 200, device="cuda")[..., ::2]        # an output whose elements lie apart
+    donnx.ONNXRMSNormalization(X=x, scale=gamma, Y=wide, epsilon=1e-5)
+    assert torch.equal(wide, y)
+    out, total = torch.empty_like(x), torch.empty_like(x)
+    donnx.ONNXSkipSimplifiedLayerNormalization(input=x, skip=skip, gamma=gamma, output=out, input_skip_bias_sum=total)
+    want = ops.rmsnorm(x, gamma, residual=skip, eps=1e-5)
+    assert torch.equal(out, want[0]) and torch.equal(total, want[1])
+    out.zero_()
+    donnx.ONNXSkipSimplifiedLayerNormalization(input=x, skip=skip, gamma=gamma, output=out)
+    assert torch.equal(out, want[0])
+    with pytest.raises(NotImplementedError, match="last axis"):
+        donnx.ONNXRMSNormalization(X=x, scale=gamma, Y=y, axis=1)
+    with pytest.raises(NotImplementedError, match="stash_type"):
+        donnx.ONNXRMSNormalization(X=x, scale=gamma, Y=y, stash_type=0)
+    with pytest.raises(ValueError, match="output connector"):
+        donnx.ONNXRMSNormalization(X=x, scale=gamma, Y=y[:2])
