@@ -94,7 +94,14 @@ __device__ __forceinline__ void load_gamma(const RowParams &p, int c, float (&g)
   } else {
     const T *q = static_cast<const T *>(p.gamma) + c;
     if constexpr (VEC == 1) {
-      g[0] = to_f32<T>(__ldg(q));  // read-only: may be loaded before h is stored
+      // Read-only, so that it may be loaded before h is stored. As an integer: the overloads of __ldg for 16-bit floats are
+      // assembly without side effects to the compiler, which may move it in front of the checks that guard it.
+      if constexpr (sizeof(T) == 4) {
+        g[0] = __ldg(reinterpret_cast<const float *>(q));
+      } else {
+        const unsigned short u = __ldg(reinterpret_cast<const unsigned short *>(q));
+        g[0] = to_f32<T>(*reinterpret_cast<const T *>(&u));
+      }
     } else {
       const uint4 u = __ldg(reinterpret_cast<const uint4 *>(q));
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
