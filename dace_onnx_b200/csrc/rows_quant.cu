@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kRowsPerCta = 8;         // rows of a CTA of the warp-per-row form
 constexpr int kMaxBlock = 1024;
+constexpr int kShiftedBlock = 576;      // of a row with ends
 constexpr int kLongBlock = 1024;
 
 struct RowParams {
@@ -156,12 +157,44 @@ __device__ __forceinline__ void join(float &sum, uint32_t &top, float *red) {
 // `top` is the pattern of max|y|: the floor keeps 448 / max finite; a NaN fails the comparison and stays.
 __device__ __forceinline__ float row_max(float top) { return top < kTinyRowMax ? kTinyRowMax : top; }
 
-// Threads of a CTA that holds a row: the registers of 8 values allow two CTAs of 1024 threads on an SM, of more one.
-constexpr int row_ctas(int values) { return values <= 8 ? 2 : 1; }
+// What both in-register kernels do with the values of one access. NORM: w is the residual; otherwise w is the gate.
+template <typename T, bool NORM, int VEC>
+__device__ __forceinline__ void combine(const RowParams &p, float (&v)[VEC], const float (&w)[VEC]) {
+  if (NORM) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] += w[i];
+  } else {
+    switch (p.activation) {  // uniform
+      case B200_ACT_RELU: gate_vec<B200_ACT_RELU, VEC>(v, w); break;
+      case B200_ACT_GELU: gate_vec<B200_ACT_GELU, VEC>(v, w); break;
+      case B200_ACT_GELU_TANH: gate_vec<B200_ACT_GELU_TANH, VEC>(v, w); break;
+      case B200_ACT_SILU: gate_vec<B200_ACT_SILU, VEC>(v, w); break;
+      default: gate_vec<B200_ACT_NONE, VEC>(v, w);
+    }
+  }
+}
 
-// The row in registers, NV accesses of VEC values a thread. NORM: z is the residual; otherwise z is the gate.
+// From the row's sum of squares and largest pattern to the factor that turns h * gamma into the output; the first thread
+// of the row stores its scale.
+template <bool NORM, bool CODES>
+__device__ __forceinline__ float row_factor(const RowParams &p, int64_t row, float sum, uint32_t top, bool first) {
+  const float rho = NORM ? 1.f / sqrtf(sum / (float)p.len + p.eps) : 1.f;
+  if (!CODES) return rho;
+  const float m = row_max(__uint_as_float(top) * rho);
+  if (first) p.scale[row] = m / kE4M3Max;
+  return rho * (kE4M3Max / m);
+}
+
+// Threads of a CTA that holds a row: the registers of 8 values allow two CTAs of 1024 threads on an SM, of more one; 16
+// values read one by one leave room for 512 threads.
+constexpr int row_ctas(int values) { return values <= 8 ? 2 : 1; }
+constexpr int row_block(int vec, int accesses) { return vec == 1 && accesses > 4 ? kMaxBlock / 2 : kMaxBlock; }
+
+// The row in registers, NV accesses of VEC values a thread. (CTAs that take several rows and load the next while they store
+// were slower, their second set of registers halves the rows in flight: 8192 x 8192 norm 73 -> 84 us, 16384 x 4096 fp32
+// rows 55 -> 77 us.)
 template <typename T, bool NORM, bool CODES, int VEC, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? kRowsPerCta * 32 : kMaxBlock, WARP ? 2 : row_ctas(VEC * NV))
+__global__ void __launch_bounds__(WARP ? kRowsPerCta * 32 : row_block(VEC, NV), WARP ? 2 : row_ctas(VEC * NV))
 rows_kernel(const RowParams p) {
   __shared__ float red[64];
   let_next_start();
@@ -193,21 +226,10 @@ rows_kernel(const RowParams p) {
     if (p.z) {
       float w[VEC];
       zr[n].get(w);
-      if (NORM) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[n][i] += w[i];
-        store_vec<T, VEC>(h + c, v[n]);
-      } else {
-        switch (p.activation) {  // uniform
-          case B200_ACT_RELU: gate_vec<B200_ACT_RELU, VEC>(v[n], w); break;
-          case B200_ACT_GELU: gate_vec<B200_ACT_GELU, VEC>(v[n], w); break;
-          case B200_ACT_GELU_TANH: gate_vec<B200_ACT_GELU_TANH, VEC>(v[n], w); break;
-          case B200_ACT_SILU: gate_vec<B200_ACT_SILU, VEC>(v[n], w); break;
-          default: gate_vec<B200_ACT_NONE, VEC>(v[n], w);
-        }
-      }
+      combine<T, NORM, VEC>(p, v[n], w);
     }
     if (NORM) {
+      if (p.z) store_vec<T, VEC>(h + c, v[n]);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sum = fmaf(v[n][i], v[n][i], sum);
       if (p.gamma) {
@@ -223,13 +245,7 @@ rows_kernel(const RowParams p) {
     }
   }
   join<WARP>(sum, top, red);
-  const float rho = NORM ? 1.f / sqrtf(sum / (float)p.len + p.eps) : 1.f;
-  float mult = rho;
-  if (CODES) {
-    const float m = row_max(__uint_as_float(top) * rho);
-    if (t == 0) p.scale[row] = m / kE4M3Max;
-    mult = rho * (kE4M3Max / m);
-  }
+  const float mult = row_factor<NORM, CODES>(p, row, sum, top, t == 0);
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
     const int c = (n * lanes + t) * VEC;
@@ -238,6 +254,115 @@ rows_kernel(const RowParams p) {
       for (int i = 0; i < VEC; ++i) v[n][i] *= mult;
       if (CODES) store_codes<VEC>(static_cast<uint8_t *>(p.y) + row * p.y_stride + c, v[n]);
       else store_vec<T, VEC>(static_cast<T *>(p.y) + row * p.y_stride + c, v[n]);
+    }
+  }
+}
+
+// Rows that do not start at multiples of 16 bytes, but all tensors of the operands' type at the same distance `off` (in values)
+// behind one, as contiguous tensors of an odd width have. Accesses are the aligned 16 bytes around the row; only its two
+// ends are read and written value by value. The codes' rows start elsewhere: they are put together in shared memory, at
+// the accesses' positions, and leave shifted by `off` bytes, sixteen at a time. A CTA is a row.
+template <typename T, bool NORM, bool CODES, int NV>
+__global__ void __launch_bounds__(kShiftedBlock)
+shifted_rows_kernel(const RowParams p) {
+  constexpr int V = 16 / (int)sizeof(T);
+  extern __shared__ __align__(16) uint32_t packed[];
+  __shared__ float red[64];
+  let_next_start();
+  wait_previous();
+  const int lanes = blockDim.x, t = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
+  const T *z = static_cast<const T *>(p.z) + (p.z ? row * p.z_stride : 0);
+  T *h = static_cast<T *>(p.h) + (p.h ? row * p.h_stride : 0);
+  const int off = (int)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+  auto first = [&](int n) { return (n * lanes + t) * V - off; };  // column of access n's first value
+  auto whole = [&](int c) { return c >= 0 && c + V <= p.len; };
+  auto read = [&](const T *q, int c, float (&v)[V]) {  // an end of the row
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = c + i >= 0 && c + i < p.len ? to_f32<T>(q[c + i]) : 0.f;
+  };
+  auto write = [&](T *q, int c, const float (&v)[V]) {
+    if (whole(c)) {
+      store_vec<T, V>(q + c, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (c + i >= 0 && c + i < p.len) q[c + i] = from_f32<T>(v[i]);
+    }
+  };
+  Raw<T, V> xr[NV], zr[NV];
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int c = first(n);
+    if (whole(c)) {
+      xr[n].load(x + c);
+      if (p.z) zr[n].load(z + c);
+    }
+  }
+  float v[NV][V];
+  float sum = 0.f;
+  uint32_t top = 0;
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int c = first(n);
+    if (c >= p.len) continue;
+    float w[V];
+    if (whole(c)) {
+      xr[n].get(v[n]);
+      if (p.z) zr[n].get(w);
+    } else {
+      read(x, c, v[n]);
+      if (p.z) read(z, c, w);
+    }
+    if (p.z) combine<T, NORM, V>(p, v[n], w);
+    if (NORM) {
+      if (p.z) write(h, c, v[n]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum = fmaf(v[n][i], v[n][i], sum);
+      if (p.gamma) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float g[1] = {0.f};
+          if (c + i >= 0 && c + i < p.len) load_gamma<T, 1>(p, c + i, g);
+          v[n][i] *= g[0];
+        }
+      }
+    }
+    if (CODES) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(v[n][i]) & 0x7fffffffu);
+    }
+  }
+  join<false>(sum, top, red);
+  const float mult = row_factor<NORM, CODES>(p, row, sum, top, t == 0);
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int c = first(n);
+    if (c >= p.len) continue;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[n][i] *= mult;
+    if (CODES) store_codes<V>(reinterpret_cast<uint8_t *>(packed) + (c + off), v[n]);
+    else write(static_cast<T *>(p.y) + row * p.y_stride, c, v[n]);
+  }
+  if (CODES) {
+    __syncthreads();
+    uint8_t *q = static_cast<uint8_t *>(p.y) + row * p.y_stride;
+    const uint32_t *word = packed + off / 4;
+    const int shift = off % 4 * 8;
+    for (int c = 16 * t; c < p.len; c += 16 * lanes) {
+      uint32_t w[5];
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = word[c / 4 + i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], shift);
+      if (c + 16 <= p.len) {
+        *reinterpret_cast<uint4 *>(q + c) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (c + i < p.len) q[c + i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+      }
     }
   }
 }
@@ -272,13 +397,7 @@ long_rows_kernel(const RowParams p) {
     if (CODES) top = max(top, __float_as_uint(times_gamma(v, c)) & 0x7fffffffu);
   }
   join<false>(sum, top, red);
-  const float rho = NORM ? 1.f / sqrtf(sum / (float)p.len + p.eps) : 1.f;
-  float mult = rho;
-  if (CODES) {
-    const float m = row_max(__uint_as_float(top) * rho);
-    if (threadIdx.x == 0) p.scale[row] = m / kE4M3Max;
-    mult = rho * (kE4M3Max / m);
-  }
+  const float mult = row_factor<NORM, CODES>(p, row, sum, top, threadIdx.x == 0);
   for (int c = threadIdx.x; c < p.len; c += blockDim.x) {
     const float v = value(c);
     const float o = times_gamma(v, c) * mult;
@@ -297,16 +416,36 @@ int launch_rows(cudaStream_t st, const RowParams &p, bool warp, int threads) {
   return launch_overlapped("rows", rows_kernel<T, NORM, CODES, VEC, NV, false>, (unsigned)p.rows, threads, 0, st, 1, p);
 }
 
+template <typename T, bool NORM, bool CODES, int NV>
+int launch_shifted(cudaStream_t st, const RowParams &p, int units) {
+  const int threads = ((units + NV - 1) / NV + 31) / 32 * 32;
+  // a row's codes from the first access on, and what the last sixteen read behind them
+  const size_t smem = CODES ? ((size_t)units * (16 / sizeof(T)) + 16 + 32) / 16 * 16 : 0;
+  return launch_overlapped("rows(shifted)", shifted_rows_kernel<T, NORM, CODES, NV>, (unsigned)p.rows, threads, smem, st, 1, p);
+}
+
+// How the rows of the operands lie: at multiples of 16 bytes, all equally far behind one, or neither.
+enum class Rows { kAligned, kShifted, kAny };
+
 template <typename T, bool NORM, bool CODES>
-int dispatch(cudaStream_t st, const RowParams &p, bool vec) {
+int dispatch(cudaStream_t st, const RowParams &p, Rows rows) {
   constexpr int V = 16 / (int)sizeof(T);
+  const bool vec = rows == Rows::kAligned;
+  const bool few = p.rows <= 2 * kNumSMs;
+  // Shorter rows, and few that a CTA of scalar accesses covers, are not worth the two ends (bf16 gate: 40000 x 511 scalar
+  // 33 us, this 64; 30000 x 701 45 and 41; 8192 x 4097 192 and 45; 100 x 1001 1.9 and 3.1; 100 x 4095 3.2 and 3.4).
+  if (rows == Rows::kShifted && p.len > (few ? 4096 : 512)) {
+    const int units = (p.len + 2 * V - 2) / V;  // aligned accesses that an unaligned row touches at most
+    if (units <= (V == 8 ? 2 * kShiftedBlock : 1024)) return launch_shifted<T, NORM, CODES, 2>(st, p, units);
+    if (units <= 4 * kShiftedBlock) return launch_shifted<T, NORM, CODES, 4>(st, p, units);
+    if (units <= 32 / V * kShiftedBlock) return launch_shifted<T, NORM, CODES, 32 / V>(st, p, units);
+  }
   const int per = vec ? V : 1;                     // values of one access
   const int units = (p.len + per - 1) / per;       // accesses of a row (len is a multiple of V when vec)
   // Accesses of a thread, measured at 6.1 to 6.5 TB/s: two (four with a gate, whose arithmetic hides behind more
   // loads), and more where the CTA would have over 512 threads (8192 x 8192 bf16 norm: 1024 threads 84 us, 512 threads
   // 73 us; 8192 x 14336 gate: 896 threads 149 us, 448 threads 107 us). Few rows leave SMs idle: one access each, for
   // the shortest way through a row. A warp takes a row that four accesses of it hold.
-  const bool few = p.rows <= 2 * kNumSMs;
   const int most = vec ? 32 / V : 16;
   const bool warp = units <= 128 && (!vec || p.rows >= kRowsPerCta * kNumSMs);
   int nv = warp ? 1 : few ? 1 : NORM || !p.z ? 2 : 4;
@@ -315,9 +454,8 @@ int dispatch(cudaStream_t st, const RowParams &p, bool vec) {
   } else {
     if (!vec) nv = 4;
     while (nv < most && nv * (few || !vec ? kMaxBlock : 512) < units) nv *= vec ? 2 : 4;
-    if (nv * kMaxBlock < units) {
+    if (nv * row_block(per, nv) < units)
       return launch_overlapped("rows(long)", long_rows_kernel<T, NORM, CODES>, (unsigned)p.rows, kLongBlock, 0, st, 1, p);
-    }
   }
   const int threads = ((units + nv - 1) / nv + 31) / 32 * 32;
   if (vec) {
@@ -335,6 +473,11 @@ int dispatch(cudaStream_t st, const RowParams &p, bool vec) {
 bool rows16(const void *p, int64_t rows, int64_t stride, int64_t elem) {
   return aligned16(p) && (rows <= 1 || (stride * elem) % 16 == 0);
 }
+// The distance of every row behind a multiple of 16 bytes follows from the base's and the stride's.
+bool same_distance(const void *p, const void *q, int64_t rows, int64_t p_stride, int64_t q_stride, int64_t elem) {
+  return (reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(q)) % 16 == 0 &&
+         (rows <= 1 || (p_stride - q_stride) * elem % 16 == 0);
+}
 bool stride_ok(int64_t stride, int64_t len, int64_t rows, bool input) {
   return stride >= len || rows <= 1 || (input && stride == 0);
 }
@@ -343,11 +486,11 @@ int type_bytes(int type) { return type == B200_TYPE_F32 ? 4 : 2; }
 bool float_type(int type) { return type == B200_TYPE_F32 || type == B200_TYPE_F16 || type == B200_TYPE_BF16; }
 
 template <bool NORM, bool CODES>
-int by_type(cudaStream_t st, int type, const RowParams &p, bool vec) {
+int by_type(cudaStream_t st, int type, const RowParams &p, Rows rows) {
   switch (type) {
-    case B200_TYPE_F32: return dispatch<float, NORM, CODES>(st, p, vec);
-    case B200_TYPE_F16: return dispatch<__half, NORM, CODES>(st, p, vec);
-    default: return dispatch<__nv_bfloat16, NORM, CODES>(st, p, vec);
+    case B200_TYPE_F32: return dispatch<float, NORM, CODES>(st, p, rows);
+    case B200_TYPE_F16: return dispatch<__half, NORM, CODES>(st, p, rows);
+    default: return dispatch<__nv_bfloat16, NORM, CODES>(st, p, rows);
   }
 }
 
@@ -380,10 +523,14 @@ extern "C" B200_API int b200_rmsnorm(void *stream, const b200_rmsnorm_desc *desc
   const bool vec = d.len % (16 / b) == 0 && rows16(x, d.rows, d.x_stride, b) &&
                    (!residual || (rows16(residual, d.rows, d.residual_stride, b) && rows16(h, d.rows, d.h_stride, b))) &&
                    (!gamma || aligned16(gamma)) && rows16(y, d.rows, d.y_stride, codes ? 1 : b);
+  auto like_x = [&](const void *q, int64_t stride) { return same_distance(q, x, d.rows, stride, d.x_stride, b); };
+  const bool shifted = (!residual || (like_x(residual, d.residual_stride) && like_x(h, d.h_stride))) &&
+                       (codes ? rows16(y, d.rows, d.y_stride, 1) : like_x(y, d.y_stride));
+  const Rows rows = vec ? Rows::kAligned : shifted ? Rows::kShifted : Rows::kAny;
   RowParams p = {d.rows, d.x_stride, d.residual_stride, d.h_stride, d.y_stride, x, residual, gamma, h, y, scale,
                  (int)d.len, d.eps, B200_ACT_NONE, gamma && d.gamma_type == B200_TYPE_F32 && d.type != B200_TYPE_F32};
-  return codes ? by_type<true, true>((cudaStream_t)stream, d.type, p, vec)
-               : by_type<true, false>((cudaStream_t)stream, d.type, p, vec);
+  return codes ? by_type<true, true>((cudaStream_t)stream, d.type, p, rows)
+               : by_type<true, false>((cudaStream_t)stream, d.type, p, rows);
 }
 
 extern "C" B200_API int b200_quantize_rows(void *stream, const b200_quantize_desc *desc, const void *x,
@@ -407,7 +554,9 @@ extern "C" B200_API int b200_quantize_rows(void *stream, const b200_quantize_des
   const int b = type_bytes(d.type);
   const bool vec = d.len % (16 / b) == 0 && rows16(x, d.rows, d.x_stride, b) && (!gate || rows16(gate, d.rows, d.gate_stride, b)) &&
                    rows16(q, d.rows, d.q_stride, 1);
+  const bool shifted = (!gate || same_distance(gate, x, d.rows, d.gate_stride, d.x_stride, b)) && rows16(q, d.rows, d.q_stride, 1);
+  const Rows rows = vec ? Rows::kAligned : shifted ? Rows::kShifted : Rows::kAny;
   RowParams p = {d.rows, d.x_stride, d.gate_stride, 0, d.q_stride, x, gate, nullptr, nullptr, q, scale,
                  (int)d.len, 0.f, d.activation, false};
-  return by_type<false, true>((cudaStream_t)stream, d.type, p, vec);
+  return by_type<false, true>((cudaStream_t)stream, d.type, p, rows);
 }

@@ -174,6 +174,36 @@ def test_strides_and_broadcast_rows(cuda):
         assert q.shape == shape and s.shape == shape[:-1] and h.shape == shape
 
 
+# a warp's and a CTA's limits; rows behind multiples of 16 bytes by every distance, all tensors by the same
+@pytest.mark.parametrize("t", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,length", [(1300, 9), (1300, 100), (1250, 249), (1200, 511), (1300, 1000), (40, 2305), (5, 4609),
+                                         (3, 9217), (2, 18001)])
+def test_rows_off_the_vector_grid(rows, length, t, cuda):
+    t = TYPES[t]
+    pitch = length | 1
+    for off in (0, 1, 6):
+        place = lambda seed: make(seed, rows * pitch + 16, t=t)[off:off + rows * pitch].view(rows, pitch)[:, :length]  # noqa: E731
+        x, r, gamma = place(30), place(31), 1 + make(32, length, scale=0.1)
+        check_norm(x, r, gamma.to(t))
+        q, s = ops.quantize_rows(x, gate=r, activation="silu")
+        check_codes(q, s, act64(r.double(), "silu") * x.double(), 2 * U, act_error(r.double(), "silu") * x.double().abs())
+        # outputs at the same distance, in place and inside a larger buffer whose other values stay
+        want = ops.rmsnorm(x, gamma, residual=r)
+        y, h = ops.rmsnorm(x, gamma, residual=r, out=torch.empty_like(want[0]), residual_out=r)
+        assert torch.equal(y, want[0]) and torch.equal(r, want[1])
+        buf = torch.full((rows * pitch + 16,), 7.0, device="cuda", dtype=t)
+        out = buf[off:off + rows * pitch].view(rows, pitch)[:, :length]
+        ops.rmsnorm(x, gamma, out=out)
+        keep = torch.ones_like(buf, dtype=torch.bool)
+        keep[off:off + rows * pitch].view(rows, pitch)[:, :length] = False
+        # not the bits of an output that lies elsewhere: another kernel may add the squares in another order, so each is within
+        # the bound of check_norm of the exact value
+        y64 = norm64(x, None, gamma, 1e-6)[1]
+        floor = torch.finfo(t).tiny * torch.finfo(t).eps
+        assert ((out.double() - y64).abs() <= (chain(length) + 1.0001 * half_step(t)) * y64.abs() + floor).all()
+        assert (buf[keep] == 7).all()
+
+
 @pytest.mark.parametrize("length", [100, 4096, 20000])
 def test_in_place_and_what_lies_behind_the_rows(length, cuda):
     x, r = make(11, 6, length, t=torch.float16), make(12, 6, length, t=torch.float16)
