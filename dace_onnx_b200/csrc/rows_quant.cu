@@ -442,21 +442,24 @@ int dispatch(cudaStream_t st, const RowParams &p, Rows rows) {
   }
   const int per = vec ? V : 1;                     // values of one access
   const int units = (p.len + per - 1) / per;       // accesses of a row (len is a multiple of V when vec)
-  // Accesses of a thread, measured at 6.1 to 6.5 TB/s: two (four with a gate, whose arithmetic hides behind more
-  // loads), and more where the CTA would have over 512 threads (8192 x 8192 bf16 norm: 1024 threads 84 us, 512 threads
-  // 73 us; 8192 x 14336 gate: 896 threads 149 us, 448 threads 107 us). Few rows leave SMs idle: one access each, for
-  // the shortest way through a row. A warp takes a row that four accesses of it hold.
-  const int most = vec ? 32 / V : 16;
-  const bool warp = units <= 128 && (!vec || p.rows >= kRowsPerCta * kNumSMs);
-  int nv = warp ? 1 : few ? 1 : NORM || !p.z ? 2 : 4;
+  // Many rows: about one CTA starts per nanosecond, so short rows are put eight to a CTA, a warp each (131072 x 256 bf16 norm
+  // 42 us, a CTA each 70; 60000 x 333 value by value 60 and 69). A longer row is a CTA's: two accesses a thread, four where
+  // one 16-bit input leaves few bytes on the way (8192 x 8192 bf16 quantise 48 -> 36 us, norm 73 either way), and more until the
+  // CTA has at most 512 threads (norm with 1024 threads 84 us), but for the spills of eight (8192 x 14336 fp32 norm 272 us, 896
+  // threads with four 235). Few rows leave SMs idle: one access each, the shortest way through a row.
+  const bool warp = units <= (!vec ? 512 : V == 4 && !p.z ? 256 : 128) && p.rows >= kRowsPerCta * kNumSMs;
+  int nv = 1;
   if (warp) {
     while (nv * 32 < units) nv *= 2;
+  } else if (vec) {
+    if (!few) nv = NORM || V == 4 ? 2 : 4;
+    while (nv < 4 && nv * (few ? kMaxBlock : 512) < units) nv *= 2;
+    if (V == 4 && nv * kMaxBlock < units) nv = 8;
   } else {
-    if (!vec) nv = 4;
-    while (nv < most && nv * (few || !vec ? kMaxBlock : 512) < units) nv *= vec ? 2 : 4;
-    if (nv * row_block(per, nv) < units)
-      return launch_overlapped("rows(long)", long_rows_kernel<T, NORM, CODES>, (unsigned)p.rows, kLongBlock, 0, st, 1, p);
+    nv = 4 * kMaxBlock < units ? 16 : 4;
   }
+  if (!warp && nv * row_block(per, nv) < units)
+    return launch_overlapped("rows(long)", long_rows_kernel<T, NORM, CODES>, (unsigned)p.rows, kLongBlock, 0, st, 1, p);
   const int threads = ((units + nv - 1) / nv + 31) / 32 * 32;
   if (vec) {
     switch (nv) {
