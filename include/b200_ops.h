@@ -5,7 +5,7 @@
  *
  * Conventions (all entry points):
  *   - every tensor pointer is a DEVICE pointer to contiguous row-major fp32 unless a stride
- *     argument says otherwise; the caller owns every buffer, the library never allocates,
+ *     argument or a `type` field says otherwise; the caller owns every buffer, the library never allocates,
  *     frees or caches device memory, and never writes its inputs (one documented exception:
  *     b200_conv2d_static_f32 keeps its scratch in a fixed array inside the library and caches that
  *     array's address per device);
