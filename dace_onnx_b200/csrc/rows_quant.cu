@@ -482,7 +482,7 @@ bool same_distance(const void *p, const void *q, int64_t rows, int64_t p_stride,
          (rows <= 1 || (p_stride - q_stride) * elem % 16 == 0);
 }
 bool stride_ok(int64_t stride, int64_t len, int64_t rows, bool input) {
-  return stride >= len || rows <= 1 || (input && stride == 0);
+  return stride >= (input ? 0 : len) || rows <= 1;
 }
 
 int type_bytes(int type) { return type == B200_TYPE_F32 ? 4 : 2; }
@@ -521,7 +521,7 @@ extern "C" B200_API int b200_rmsnorm(void *stream, const b200_rmsnorm_desc *desc
   if (!residual != !h) return fail(B200_EINVAL, "rmsnorm: residual and h come together");
   if (!stride_ok(d.x_stride, d.len, d.rows, true) || (residual && !stride_ok(d.residual_stride, d.len, d.rows, true)) ||
       (h && !stride_ok(d.h_stride, d.len, d.rows, false)) || !stride_ok(d.y_stride, d.len, d.rows, false))
-    return fail(B200_EINVAL, "rmsnorm: a row stride is smaller than the row");
+    return fail(B200_EINVAL, "rmsnorm: an input's row stride is negative, or an output's smaller than the row");
   const int b = type_bytes(d.type);
   const bool vec = d.len % (16 / b) == 0 && rows16(x, d.rows, d.x_stride, b) &&
                    (!residual || (rows16(residual, d.rows, d.residual_stride, b) && rows16(h, d.rows, d.h_stride, b))) &&
@@ -553,7 +553,7 @@ extern "C" B200_API int b200_quantize_rows(void *stream, const b200_quantize_des
   if (!x || !q || !scale) return fail(B200_EINVAL, "quantize_rows: null pointer");
   if (!stride_ok(d.x_stride, d.len, d.rows, true) || (gate && !stride_ok(d.gate_stride, d.len, d.rows, true)) ||
       !stride_ok(d.q_stride, d.len, d.rows, false))
-    return fail(B200_EINVAL, "quantize_rows: a row stride is smaller than the row");
+    return fail(B200_EINVAL, "quantize_rows: an input's row stride is negative, or the output's smaller than the row");
   const int b = type_bytes(d.type);
   const bool vec = d.len % (16 / b) == 0 && rows16(x, d.rows, d.x_stride, b) && (!gate || rows16(gate, d.rows, d.gate_stride, b)) &&
                    rows16(q, d.rows, d.q_stride, 1);

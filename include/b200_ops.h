@@ -261,9 +261,9 @@ B200_API int b200_maxpool2d_f32(void *stream, const float *x, float *y, int64_t 
  *
  * These entry points take typed tensors: `type` fields hold a B200_TYPE_* code. Row i of a tensor starts
  * stride * i elements after its base, elements of a row are adjacent; any natural alignment is accepted unless an
- * entry point says otherwise (16-byte aligned bases and rows take the 128-bit accesses). An input's row
- * stride may be 0 (one row used for all). An output may be exactly the same rows as an input of the same type
- * (same base and stride); overlapping otherwise is undefined.
+ * entry point says otherwise (16-byte aligned bases and rows take the 128-bit accesses). An input's rows may
+ * overlap, down to stride 0 (one row used for all). An output of the row operators may be exactly the same rows as an input
+ * of the same type (same base and stride), and a product's Y its residual; overlapping otherwise is undefined.
  * ------------------------------------------------------------------------------------------ */
 #define B200_TYPE_F32 0
 #define B200_TYPE_F16 1

@@ -1,4 +1,8 @@
 """The operators of the 8-bit path one after the other, as a model runs them, with buffers that the next step reuses."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -139,3 +143,76 @@ def test_norm_nodes(cuda):
         donnx.ONNXRMSNormalization(X=x, scale=gamma, Y=y, stash_type=0)
     with pytest.raises(ValueError, match="output connector"):
         donnx.ONNXRMSNormalization(X=x, scale=gamma, Y=y[:2])
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    """Nothing that a first call sets up (attributes, addresses, modules) keeps it from being captured."""
+    code = """
+import torch
+from dace_onnx_b200 import ops
+x, w = torch.randn(300, 256, device="cuda"), torch.randn(512, 256, device="cuda")
+wide, few = torch.randn(2, 256, 512, device="cuda").bfloat16()[0], torch.randn(3, 512, device="cuda").bfloat16()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    q, s = ops.rmsnorm_quantize(x)
+    qw, sw = ops.quantize_rows(w)
+    y = ops.matmul_scaled(q, qw, a_scale=s, w_scale=sw, out_dtype=torch.float32)
+    z = ops.matmul_scaled(few, wide)
+graph.replay()
+torch.cuda.synchronize()
+q2, s2 = ops.rmsnorm_quantize(x)
+assert torch.equal(ops.matmul_scaled(q2, qw, a_scale=s2, w_scale=sw, out_dtype=torch.float32), y)
+assert torch.equal(ops.matmul_scaled(few, wide), z)
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_fork_and_join_inside_a_capture(cuda):
+    """Two branches of a captured step on two streams, joined by a third call that reads both."""
+    x, a, b = make(100, 40, 512).bfloat16(), ops.PreparedLinear(make(101, 512, 512)), ops.PreparedLinear(make(102, 512, 512))
+    side = torch.cuda.Stream()
+
+    def step():
+        q, s = ops.quantize_rows(x)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            u = b(q, a_scale=s, out_dtype=torch.bfloat16)
+        v = a(q, a_scale=s, out_dtype=torch.bfloat16)
+        torch.cuda.current_stream().wait_stream(side)
+        return ops.rmsnorm(v, residual=u)
+
+    want = step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(20):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_written_weights_are_seen_by_the_next_product(cuda):
+    """A product right behind the kernels that write its operands, over and over with other values in the same memory."""
+    q, s = ops.empty_codes((6, 4096), "cuda"), torch.empty(6, device="cuda")
+    qw, sw = ops.empty_codes((512, 4096), "cuda"), torch.empty(512, device="cuda")
+    xs, ws = [make(110 + i, 6, 4096) for i in range(4)], [make(120 + i, 512, 4096) for i in range(4)]
+    want = []
+    for x, w in zip(xs, ws):
+        ops.quantize_rows(x, out=q, scale=s)
+        ops.quantize_rows(w, out=qw, scale=sw)
+        torch.cuda.synchronize()
+        want.append(ops.matmul_scaled(q, qw, a_scale=s, w_scale=sw).clone())
+        torch.cuda.synchronize()
+    got = [torch.empty_like(want[0]) for _ in range(80)]
+    for i, y in enumerate(got):
+        ops.quantize_rows(xs[i % 4], out=q, scale=s)
+        ops.quantize_rows(ws[i % 4], out=qw, scale=sw)
+        ops.matmul_scaled(q, qw, a_scale=s, w_scale=sw, out=y)
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i % 4])

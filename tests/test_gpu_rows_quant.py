@@ -164,6 +164,10 @@ def test_strides_and_broadcast_rows(cuda):
         check_norm(x, g, None)
     row = make(8, 128, t=torch.bfloat16)
     check_norm(wide[:, :128], row.expand(12, 128), None)                    # row stride 0
+    windows = make(17, 400).as_strided((12, 64), (24, 1))                   # rows that overlap
+    check_norm(windows, windows, None)
+    q, s = ops.quantize_rows(windows)
+    check_codes(q, s, windows.double(), 0.0)
     x3 = make(9, 2, 3, 5, 64)
     check_norm(x3, x3 * 2, None)
     check_norm(x3.permute(1, 0, 2, 3), None, None)                          # leading axes that do not merge: copied

@@ -23,7 +23,7 @@ def test_cpu_tensors_are_refused():
 @pytest.mark.parametrize("change,args,code", [
     (dict(rows=-1), {}, _lib.EINVAL), (dict(len=0), {}, _lib.EINVAL), (dict(type=3), {}, _lib.EINVAL),
     (dict(gamma_type=2), {}, _lib.EINVAL), (dict(y_type=2), {}, _lib.EINVAL), (dict(eps=-1.0), {}, _lib.EINVAL),
-    (dict(eps=float("nan")), {}, _lib.EINVAL), (dict(x_stride=7), {}, _lib.EINVAL), (dict(y_stride=0), {}, _lib.EINVAL),
+    (dict(eps=float("nan")), {}, _lib.EINVAL), (dict(x_stride=-1), {}, _lib.EINVAL), (dict(y_stride=0), {}, _lib.EINVAL),
     (dict(h_stride=0), {}, _lib.EINVAL), (dict(rows=1 << 31), {}, _lib.EUNSUPPORTED), (dict(len=1 << 31), {}, _lib.EUNSUPPORTED),
     ({}, dict(x=None), _lib.EINVAL), ({}, dict(h=None), _lib.EINVAL), ({}, dict(residual=None), _lib.EINVAL),
     ({}, dict(y=None), _lib.EINVAL), (dict(y_type=3), dict(scale=None), _lib.EINVAL), (dict(rows=0), dict(x=None), _lib.OK)])
@@ -39,7 +39,7 @@ def test_rmsnorm_refusals(change, args, code):
 
 @pytest.mark.parametrize("change,args,code", [
     (dict(rows=-1), {}, _lib.EINVAL), (dict(len=0), {}, _lib.EINVAL), (dict(type=3), {}, _lib.EINVAL),
-    (dict(activation=5), {}, _lib.EINVAL), (dict(activation=-1), {}, _lib.EINVAL), (dict(gate_stride=7), {}, _lib.EINVAL),
+    (dict(activation=5), {}, _lib.EINVAL), (dict(activation=-1), {}, _lib.EINVAL), (dict(gate_stride=-1), {}, _lib.EINVAL),
     (dict(q_stride=0), {}, _lib.EINVAL), (dict(rows=1 << 31), {}, _lib.EUNSUPPORTED), ({}, dict(x=None), _lib.EINVAL),
     ({}, dict(gate=None), _lib.EINVAL), ({}, dict(q=None), _lib.EINVAL), ({}, dict(scale=None), _lib.EINVAL),
     (dict(rows=0), dict(x=None), _lib.OK)])
