@@ -17,8 +17,12 @@
 //          whose rows the pair kernel's vector accesses cannot address.
 //
 // The tensor core adds into its fp32 accumulator with truncation, an error that grows with the number of additions. For
-// 16-bit outputs it stays far below their rounding; for fp32 outputs the sum is cut into chunks of kChunkKb K-blocks
-// whose accumulators the epilogue warps add in registers, rounding to nearest.
+// 16-bit outputs it stays far below their rounding; for fp32 outputs the sum is cut into chunks of kChunkKb K-blocks whose
+// accumulators the epilogue warps add in registers, rounding to nearest. The shorter the chunks, the sooner the issuing warp
+// runs out of accumulators while the epilogue stores (16384 x 4096 x 1024 to fp32, 16 and 32 additions: bf16 221K and 183K cycles,
+// e4m3 143K and 127K). Products of codes are short and lose little: with 32 additions the outputs are within 1.5e-7 of 64 bits
+// (2-norm, up to K = 16384, terms of one sign too). 16-bit operands lose more (32 additions: fp16 6.5e-7, terms of one sign
+// 2.5e-6) and keep 16.
 //
 // Every mbarrier wait is bounded by a cycle budget, as in gemm_tcgen05.cu.
 #include <cuda.h>
@@ -36,7 +40,8 @@ namespace {
 constexpr int kRowBytes = 128;                    // bytes of K of one K-block
 constexpr int kTileBytes = 128 * kRowBytes;       // 128 rows of a K-block
 constexpr int kMmasPerKb = 4;                     // 32 bytes of K per instruction
-constexpr int kChunkKb = 4;                       // K-blocks of one in-core sum of fp32 outputs: 16 additions
+template <bool F8>
+constexpr int kChunkKb = F8 ? 8 : 4;              // K-blocks of one in-core sum of fp32 outputs: 32 or 16 additions
 
 struct ScaledParams {
   int64_t M, N;
@@ -205,17 +210,23 @@ __device__ __forceinline__ void teardown_after_abort(int aborted) {
 // ---------------------------------------------------------------------------------------------
 // pair
 // ---------------------------------------------------------------------------------------------
-template <int BN>
+template <int BN, typename OUT>
 struct PairCfg {
+  static constexpr bool kChunked = std::is_same<OUT, float>::value;
   static constexpr int kStageBytes = kTileBytes + BN / 2 * kRowBytes;  // 128 rows of A, half of the tile's rows of W
-  static constexpr int kStages = (160 * 1024) / kStageBytes;
-  static constexpr int kTmemCols = 2 * BN;
+  // fp32 outputs leave in twice as many blocks: two under way take the place of the fifth stage
+  static constexpr int kBlocks = kChunked || BN == 128 ? 2 : 1;
+  static constexpr int kStages = BN == 128 ? 6 : kChunked ? 4 : 5;
+  static constexpr int kAccs = kChunked ? 512 / BN : 2;    // accumulators
+  static constexpr int kTmemCols = kAccs * BN;
   static constexpr int kColsPerWarp = BN / 4;              // four warps on each quarter of the lanes
   static constexpr int kEpilogueWarps = 16;
   static constexpr int kThreads = 32 * (2 + kEpilogueWarps);
   static constexpr int kStoreBytes = 32 * 64;              // a warp's block of outputs: 32 rows of 64 bytes
   static constexpr int kVectorBytes = kColsPerWarp * 2 * 4;  // a warp's scales and biases
-  static constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * (kStoreBytes + kVectorBytes) + 1024 + 256;
+  static constexpr int kSmemBytes =
+      kStages * kStageBytes + kEpilogueWarps * (kBlocks * kStoreBytes + kVectorBytes) + 1024 + 256;
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory of an SM");
 };
 
 // Tiles in groups of eight row tiles, column tiles across a group: the ~74 tiles in flight then share about 8 + 9 tile
@@ -231,22 +242,22 @@ __device__ __forceinline__ void tile_at(const ScaledParams &p, int64_t tile, int
 }
 
 template <bool F8, typename OUT, int BN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN, OUT>::kThreads, 1)
 scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                    const __grid_constant__ CUtensorMap map_y, const ScaledParams p) {
-  using C = PairCfg<BN>;
-  constexpr bool kChunked = std::is_same<OUT, float>::value;
+  using C = PairCfg<BN, OUT>;
+  constexpr bool kChunked = C::kChunked;
   constexpr int kStages = C::kStages;
   constexpr int kKbElems = F8 ? 128 : 64;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t *store_smem = smem + kStages * C::kStageBytes;
-  uint8_t *vector_smem = store_smem + C::kEpilogueWarps * C::kStoreBytes;
+  uint8_t *vector_smem = store_smem + C::kEpilogueWarps * C::kBlocks * C::kStoreBytes;
   uint64_t *bars = reinterpret_cast<uint64_t *>(vector_smem + C::kEpilogueWarps * C::kVectorBytes);
   const uint32_t bar_full = smem_u32(bars);
   const uint32_t bar_empty = bar_full + 8 * kStages;
   const uint32_t bar_tfull = bar_empty + 8 * kStages;
-  const uint32_t bar_tempty = bar_tfull + 16;
+  const uint32_t bar_tempty = bar_tfull + 8 * C::kAccs;
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
 
@@ -265,7 +276,7 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       mbar_init(bar_full + 8 * s, 1);   // even CTA: its expect_tx for the bytes of both
       mbar_init(bar_empty + 8 * s, 1);  // each CTA: the issuer commits to both
     }
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < C::kAccs; ++a) {
       mbar_init(bar_tfull + 8 * a, 1);                       // each CTA: the issuer commits to both
       mbar_init(bar_tempty + 8 * a, 2 * C::kEpilogueWarps);  // even CTA: one arrival per epilogue warp of both
     }
@@ -318,7 +329,7 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       const uint64_t a_desc0 = make_smem_desc(smem_base, 16, 1024, kLayoutSw128);
       const uint64_t w_desc0 = make_smem_desc(smem_base + kTileBytes, 16, 1024, kLayoutSw128);
       const uint32_t idesc = p.idesc;
-      const int chunk = kChunked ? kChunkKb : p.num_kb;
+      const int chunk = kChunked ? kChunkKb<F8> : p.num_kb;
       int s = 0, acc = 0;
       uint32_t ph = 0, acc_ph = 0;
       bool ok = true;
@@ -346,7 +357,7 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             __syncwarp();
             if (++s == kStages) { s = 0; ph ^= 1; }
           }
-          if (++acc == 2) { acc = 0; acc_ph ^= 1; }
+          if (++acc == C::kAccs) { acc = 0; acc_ph ^= 1; }
         }
       }
     }
@@ -356,10 +367,11 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     float *sw = reinterpret_cast<float *>(vector_smem + ew * C::kVectorBytes), *bs = sw + C::kColsPerWarp;
     // the block of outputs on its way to memory: rows of 64 bytes whose 16-byte pieces are exchanged as the 64-byte
     // swizzle of map_y has them, so that a warp's 16-byte accesses meet no bank twice
-    const uint32_t block = smem_u32(store_smem + ew * C::kStoreBytes);
-    const uint32_t my_row = block + lane * 64, flip = (lane >> 1) & 3;
+    const uint32_t blocks = smem_u32(store_smem + ew * C::kBlocks * C::kStoreBytes);
+    const uint32_t flip = (lane >> 1) & 3;
+    int turn = 0;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + col0;
-    const int chunks = kChunked ? (p.num_kb + kChunkKb - 1) / kChunkKb : 1;
+    const int chunks = kChunked ? (p.num_kb + kChunkKb<F8> - 1) / kChunkKb<F8> : 1;
     constexpr int B = kBlockCols<OUT>;
     int acc = 0;
     uint32_t acc_ph = 0;
@@ -385,7 +397,9 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         const int64_t left = p.N - n0 - c;
         if (left <= 0 || m0 >= p.M) return;  // uniform
         const int cols = left < B ? (int)left : B;
-        if (lane == 0) bulk_wait_read();  // the previous block has left
+        const uint32_t block = blocks + turn * C::kStoreBytes, my_row = block + lane * 64;
+        if (C::kBlocks > 1) turn ^= 1;
+        if (lane == 0) bulk_wait_read<C::kBlocks - 1>();  // what was in this block has left
         __syncwarp();
         if (p.residual) finish_block<OUT, true>(p, v, sa, sw + c, bs + c, r ? r + c : nullptr, cols, my_row, flip);
         else finish_block<OUT, false>(p, v, sa, sw + c, bs + c, nullptr, cols, my_row, flip);
@@ -412,7 +426,7 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(bar_tempty + 8 * acc, 0));
-          if (++acc == 2) { acc = 0; acc_ph ^= 1; }
+          if (++acc == C::kAccs) { acc = 0; acc_ph ^= 1; }
         }
         if (!ok) break;
 #pragma unroll
@@ -435,7 +449,7 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(t[j]);
           emit(v, c);
         }
-        if (++acc == 2) { acc = 0; acc_ph ^= 1; }
+        if (++acc == C::kAccs) { acc = 0; acc_ph ^= 1; }
       }
     }
     if (lane == 0) bulk_wait();
@@ -670,7 +684,7 @@ scaled_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     const uint64_t w_desc0 = make_smem_desc(smem_base, 16, 1024, kLayoutSw128);
     const uint64_t a_desc0 = make_smem_desc(smem_base + kTileBytes, 16, 1024, kLayoutSw128);
     const uint32_t idesc = p.idesc;
-    const int chunk = kChunked ? kChunkKb : p.num_kb;
+    const int chunk = kChunked ? kChunkKb<F8> : p.num_kb;
     int s = 0, acc = 0;
     uint32_t ph = 0, acc_ph = 0;
     bool ok = true;
@@ -703,7 +717,7 @@ scaled_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     const int ew = warp - 2, quarter = warp & 3;
     const int col0 = (ew >> 2) * C::kColsPerWarp;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + col0;
-    const int chunks = kChunked ? (kb_end - kb_begin + kChunkKb - 1) / kChunkKb : 1;
+    const int chunks = kChunked ? (kb_end - kb_begin + kChunkKb<F8> - 1) / kChunkKb<F8> : 1;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int64_t n = n0 + (vec ? 4 * lane + k : lane + 32 * k);
@@ -786,7 +800,7 @@ struct Operands {
 
 template <bool F8, typename OUT, int BN>
 int launch_pair(cudaStream_t st, const Operands &o, ScaledParams &p) {
-  using C = PairCfg<BN>;
+  using C = PairCfg<BN, OUT>;
   auto kern = scaled_pair_kernel<F8, OUT, BN>;
   static std::atomic<uint64_t> smem_set{0};
   if (int rc = raise_smem(kern, C::kSmemBytes, smem_set)) return rc;

@@ -2,8 +2,8 @@
 
 Tolerances, from the arithmetic (u = 2^-24; S = sum_k |a w| with its scales):
   sum    an addition into the tensor core's accumulator truncates: at most 2u of S each. One instruction takes 32 (codes) or
-         16 values of K; fp32 outputs start a new accumulator every 16 instructions and add these rounding to nearest, and
-         K may be split over 8 CTAs
+         16 values of K; fp32 outputs start a new accumulator every 32 (codes) or 16 instructions and add these rounding to
+         nearest, and K may be split over 8 CTAs
   scales, bias: 3 roundings; activations: the bounds of act_error in test_gpu_rows_quant, slope at most 1.13
   result one rounding to its type: half a step
 """
@@ -32,9 +32,10 @@ def check(y, a, sa, w, sw, bias=None, act=None, residual=None):
     wide = lambda v, s: v.double() if s is None else v.double() * s.double().reshape(-1, 1)  # noqa: E731
     a64, w64 = wide(a.reshape(-1, k), sa), wide(w, sw)
     pre, size = a64 @ w64.t(), a64.abs() @ w64.abs().t()
-    adds = -(-k // (32 if a.dtype == torch.float8_e4m3fn else 16))
+    codes = a.dtype == torch.float8_e4m3fn
+    adds = -(-k // (32 if codes else 16))
     if y.dtype == torch.float32:
-        adds = 16 + 8 + -(-adds // 16)
+        adds = (32 if codes else 16) + 8 + -(-adds // (32 if codes else 16))
     err = (adds * 2 * U + 3 * U) * size
     if bias is not None:
         pre = pre + bias.double()
