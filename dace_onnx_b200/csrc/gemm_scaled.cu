@@ -7,14 +7,17 @@
 // Two kernels, both TMA -> shared memory -> tcgen05.mma -> TMEM -> registers, warp-specialised (one loading thread, one
 // issuing thread, epilogue warps), K-blocks of 128 bytes with the 128-byte swizzle:
 //
-//   pair   many rows of A. A cluster of two CTAs computes 256 x BN outputs (rows of A are TMEM lanes), persistent, two
-//          accumulators so that the epilogue of a tile runs under the MMAs of the next.
+//   pair   many rows of A. A cluster of two CTAs computes 256 x BN outputs (rows of A are TMEM lanes), persistent, several
+//          accumulators so that the epilogue of a tile runs under the MMAs of the next. Outputs leave through shared memory and
+//          TMA stores: 32-byte stores of each thread's own row took a third of the epilogue. Bound by the power limit: 8192 x
+//          14336, K 4096, e4m3 with bias and silu 390 us (2.47 PFLOP/s) at 1000 W and 1.1 to 1.2 GHz.
 //   split  few rows of A, where the weights' bytes bound the product and there are fewer tiles than SMs. Operands
 //          change places: 128 rows of W are the TMEM lanes and NT rows of A the columns, so that a single token fills
 //          the tensor core's wide side with weights. K is split over the CTAs of a cluster (at most 8), whose partial
 //          sums meet in distributed shared memory in a fixed order (the same bits every time, no workspace). Lanes of
 //          a warp write neighbouring columns of Y, so its stores are dense at any alignment: it also takes outputs
-//          whose rows the pair kernel's vector accesses cannot address.
+//          whose rows the pair kernel's vector accesses cannot address. Bound by memory and by its start and end: 32 x 28672,
+//          K 4096, e4m3 23 us (5.2 TB/s); one row, 4096 x 4096, 6 us.
 //
 // The tensor core adds into its fp32 accumulator with truncation, an error that grows with the number of additions. For
 // 16-bit outputs it stays far below their rounding; for fp32 outputs the sum is cut into chunks of kChunkKb K-blocks whose
