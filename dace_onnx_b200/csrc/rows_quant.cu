@@ -10,9 +10,9 @@
 // over the registers and joined in one exchange between warps. The maximum runs on the bit patterns of |y| as
 // unsigned integers: they order like the values, and a NaN's pattern is above infinity's, so a NaN reaches the scale.
 //
-// Measured over three sets of data in rotation (bytes read and written once / time): 8192 x 8192 bf16 norm with residual to e4m3 78
-// us, 6.0 TB/s; 16384 x 1024 fp32 the same 37 us, 5.9 TB/s; 8192 x 14336 bf16 silu(gate) * x 109 us, 5.4 TB/s; 16384 x 4096 fp32
-// 60 us, 5.6 TB/s. A copy runs at 6.5 TB/s.
+// Measured over three sets of data in rotation (bytes read and written once / time): 8192 x 8192 bf16 norm with residual to e4m3 76
+// us, 6.2 TB/s; 16384 x 1024 fp32 the same 36 us, 6.0 TB/s; 8192 x 14336 bf16 silu(gate) * x 103 us, 5.7 TB/s; 16384 x 4096 fp32
+// 57 us, 5.9 TB/s. A copy runs at 6.5 TB/s.
 #include <math.h>
 
 #include "typed.cuh"
