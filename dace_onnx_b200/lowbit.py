@@ -13,8 +13,14 @@ import ctypes
 
 import torch
 
-from . import _lib, torch_calls
+from . import _lib
 from ._lib import ACTIVATIONS, TYPE_BF16, TYPE_E4M3, TYPE_F16, TYPE_F32, GemmScaledDesc, QuantizeDesc, RmsnormDesc, check
+
+try:
+    from . import torch_calls
+except ImportError as e:
+    raise ImportError("dace_onnx_b200/torch_calls.so is missing or does not fit this torch: build it with "
+                      "`python -m dace_onnx_b200.build` (%s)" % e) from e
 
 FLOAT_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
 E4M3 = torch.float8_e4m3fn
