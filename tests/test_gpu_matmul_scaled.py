@@ -86,6 +86,15 @@ def test_every_plan(m, n, k, cuda):
         check(ops.matmul_scaled(a, w, a_scale=sa, w_scale=sw, bias=bias, residual=residual), a, sa, w, sw, bias, None, residual)
 
 
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("m,n,k", [(3055, 919, 5536), (3055, 920, 5536), (40, 1001, 16392)])
+def test_long_sums_to_fp32(m, n, k, t, cuda):
+    """Many accumulators one after the other, on rows that vector accesses can address and not."""
+    a, _, w, _ = operands(m, n, k, TYPES[t])
+    bias = make(5, n)
+    check(ops.matmul_scaled(a, w, bias=bias, activation="gelu_tanh", out_dtype=torch.float32), a, None, w, None, bias, "gelu_tanh")
+
+
 @pytest.mark.parametrize("act", [None, "relu", "gelu", "gelu_tanh", "silu"])
 @pytest.mark.parametrize("m,n", [(5, 333), (300, 512)])
 def test_epilogues(m, n, act, cuda):
