@@ -61,19 +61,22 @@ struct ScaledParams {
   unsigned *status;
 };
 
+// Scales and bias may be what the kernel before this one in the stream has just written, and that kernel was still running when
+// this one started: plain loads behind wait_previous(). The read-only path (__ldg) asks for data that nobody writes while the
+// kernel exists; neither its cache nor the compiler is bound by the wait.
 __device__ __forceinline__ float bias_at(const ScaledParams &p, int64_t n) {
   if (!p.bias) return 0.f;
   switch (p.bias_type) {
-    case B200_TYPE_F32: return __ldg(static_cast<const float *>(p.bias) + n);
+    case B200_TYPE_F32: return static_cast<const float *>(p.bias)[n];
     case B200_TYPE_F16: return __half2float(static_cast<const __half *>(p.bias)[n]);
     default: return __bfloat162float(static_cast<const __nv_bfloat16 *>(p.bias)[n]);
   }
 }
 __device__ __forceinline__ float w_scale_at(const ScaledParams &p, int64_t n) {
-  return p.w_scale ? __ldg(p.w_scale + n * p.w_scale_step) : 1.f;
+  return p.w_scale ? p.w_scale[n * p.w_scale_step] : 1.f;
 }
 __device__ __forceinline__ float a_scale_at(const ScaledParams &p, int64_t m) {
-  return p.a_scale ? __ldg(p.a_scale + m * p.a_scale_step) : 1.f;
+  return p.a_scale ? p.a_scale[m * p.a_scale_step] : 1.f;
 }
 
 // 32 bytes of a row of the residual, in one access or two

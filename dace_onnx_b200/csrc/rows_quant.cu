@@ -82,33 +82,29 @@ __device__ __forceinline__ void store_codes(uint8_t *p, const float (&v)[VEC]) {
     *reinterpret_cast<uint2 *>(p) = make_uint2(e4m3x2(v[0], v[1]) | e4m3x2(v[2], v[3]) << 16,
                                                e4m3x2(v[4], v[5]) | e4m3x2(v[6], v[7]) << 16);
 }
-// gamma, read by every row: cached loads
+// gamma, read by every row: cached loads, but not those of the read-only path (__ldg). That path asks for data that nobody
+// writes while the kernel exists, and the kernel before this one, which may write gamma, still runs when this one starts; the loads
+// of 16-bit floats among its functions are also assembly without side effects to the compiler, which may move it in front of
+// the checks that guard it.
 template <typename T, int VEC>
 __device__ __forceinline__ void load_gamma(const RowParams &p, int c, float (&g)[VEC]) {
   if (p.gamma_f32) {
     const float *q = static_cast<const float *>(p.gamma) + c;
     if constexpr (VEC == 1) {
-      g[0] = __ldg(q);
+      g[0] = *q;
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; i += 4) {
-        const float4 f = __ldg(reinterpret_cast<const float4 *>(q + i));
+        const float4 f = *reinterpret_cast<const float4 *>(q + i);
         g[i] = f.x; g[i + 1] = f.y; g[i + 2] = f.z; g[i + 3] = f.w;
       }
     }
   } else {
     const T *q = static_cast<const T *>(p.gamma) + c;
     if constexpr (VEC == 1) {
-      // Read-only, so that it may be loaded before h is stored. As an integer: the overloads of __ldg for 16-bit floats are
-      // assembly without side effects to the compiler, which may move it in front of the checks that guard it.
-      if constexpr (sizeof(T) == 4) {
-        g[0] = __ldg(reinterpret_cast<const float *>(q));
-      } else {
-        const unsigned short u = __ldg(reinterpret_cast<const unsigned short *>(q));
-        g[0] = to_f32<T>(*reinterpret_cast<const T *>(&u));
-      }
+      g[0] = to_f32<T>(*q);
     } else {
-      const uint4 u = __ldg(reinterpret_cast<const uint4 *>(q));
+      const uint4 u = *reinterpret_cast<const uint4 *>(q);
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -233,12 +229,12 @@ rows_kernel(const RowParams p) {
       combine<T, NORM, VEC>(p, v[n], w);
     }
     if (NORM) {
+      float g[VEC];
+      if (p.gamma) load_gamma<T, VEC>(p, c, g);
       if (p.z) store_vec<T, VEC>(h + c, v[n]);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sum = fmaf(v[n][i], v[n][i], sum);
       if (p.gamma) {
-        float g[VEC];
-        load_gamma<T, VEC>(p, c, g);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[n][i] *= g[i];
       }
