@@ -174,27 +174,62 @@ __device__ __forceinline__ void combine(const RowParams &p, float (&v)[VEC], con
   }
 }
 
-// From the row's sum of squares and largest pattern to the factor that turns h * gamma into the output; the first thread
-// of the row stores its scale.
+// What turns h * gamma (or y itself) into the output: y = v * rho, and code = y / scale. The two are not one factor: 448 / max alone
+// is up to 5.7e32 (rows of zeros), which times rho overflows once eps is below 3e-12; and the product y * (448 / max) is not
+// the quotient y / scale where that lies at a tie of e4m3, which for 16-bit inputs it often does.
+//
+// The quotient takes one reciprocal a row: q = y * inv, corrected once by its remainder, q + (y - q * scale) * inv (Markstein, IBM J.
+// Res. Dev. 34, 1990). The remainder is exact but for its last bit, so the sum is y / scale to within 2^-45 before its one
+// rounding. (A division for every value: 8192 x 14336 gate 108 -> 140 us.)
+struct RowFactor {
+  float rho, inv, minus_scale;
+};
+// From the row's sum of squares and largest pattern; the first thread of the row stores its scale.
 template <bool NORM, bool CODES>
-__device__ __forceinline__ float row_factor(const RowParams &p, int64_t row, float sum, uint32_t top, bool first) {
+__device__ __forceinline__ RowFactor row_factor(const RowParams &p, int64_t row, float sum, uint32_t top, bool first) {
   const float rho = NORM ? 1.f / sqrtf(sum / (float)p.len + p.eps) : 1.f;
-  if (!CODES) return rho;
-  const float m = row_max(__uint_as_float(top) * rho);
-  if (first) p.scale[row] = m / kE4M3Max;
-  return rho * (kE4M3Max / m);
+  if (!CODES) return RowFactor{rho, 1.f, 0.f};
+  const float scale = row_max(__uint_as_float(top) * rho) / kE4M3Max;
+  if (first) p.scale[row] = scale;
+  // an infinite scale makes quotients of finite values 0, which need no correction (and 0 * inf would be none)
+  return RowFactor{rho, 1.f / scale, scale == INFINITY ? 0.f : -scale};
+}
+template <bool NORM, bool CODES, int VEC>
+__device__ __forceinline__ void finish(const RowFactor &f, float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    if (NORM) v[0] *= f.rho;
+    if (CODES) {
+      const float q = v[0] * f.inv;
+      v[0] = fmaf(fmaf(q, f.minus_scale, v[0]), f.inv, q);
+    }
+  } else {
+    const Pair rho = both(f.rho), inv = both(f.inv), minus_scale = both(f.minus_scale);
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      Pair y(v[i], v[i + 1]);
+      if (NORM) y = y * rho;
+      if (CODES) {
+        const Pair q = y * inv;
+        y = fma2(fma2(q, minus_scale, y), inv, q);
+      }
+      y.get(v[i], v[i + 1]);
+    }
+  }
 }
 
-// Threads of a CTA that holds a row: the registers of 8 values allow two CTAs of 1024 threads on an SM, of more one; 16
-// values read one by one leave room for 512 threads.
-constexpr int row_ctas(int values) { return values <= 8 ? 2 : 1; }
+// Registers of a thread. A CTA that holds a row has up to 1024 threads: those of at most 8 values share an SM with another such CTA,
+// and 16 values in two accesses, which run as CTAs of up to 512 threads, leave room for three of them (8192 x 8192 bf16 norm with
+// 45 registers, two CTAs 87 us, with 40 77). 16 values read one by one take up to 128 and 512 threads.
 constexpr int row_block(int vec, int accesses) { return vec == 1 && accesses > 4 ? kMaxBlock / 2 : kMaxBlock; }
+constexpr int row_registers(int vec, int accesses, bool warp) {
+  return warp || row_block(vec, accesses) < kMaxBlock ? 128 : vec * accesses <= 8 ? 32 : accesses == 2 ? 40 : 64;
+}
 
 // The row in registers, NV accesses of VEC values a thread. (CTAs that take several rows and load the next while they store
 // were slower, their second set of registers halves the rows in flight: 8192 x 8192 norm 73 -> 84 us, 16384 x 4096 fp32
 // rows 55 -> 77 us.)
 template <typename T, bool NORM, bool CODES, int VEC, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? kRowsPerCta * 32 : row_block(VEC, NV), WARP ? 2 : row_ctas(VEC * NV))
+__global__ void __maxnreg__(row_registers(VEC, NV, WARP))
 rows_kernel(const RowParams p) {
   __shared__ float red[64];
   let_next_start();
@@ -245,13 +280,12 @@ rows_kernel(const RowParams p) {
     }
   }
   join<WARP>(sum, top, red);
-  const float mult = row_factor<NORM, CODES>(p, row, sum, top, t == 0);
+  const RowFactor factor = row_factor<NORM, CODES>(p, row, sum, top, t == 0);
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
     const int c = (n * lanes + t) * VEC;
     if (c < p.len) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[n][i] *= mult;
+      finish<NORM, CODES, VEC>(factor, v[n]);
       if (CODES) store_codes<VEC>(static_cast<uint8_t *>(p.y) + row * p.y_stride + c, v[n]);
       else store_vec<T, VEC>(static_cast<T *>(p.y) + row * p.y_stride + c, v[n]);
     }
@@ -335,13 +369,12 @@ shifted_rows_kernel(const RowParams p) {
     }
   }
   join<false>(sum, top, red);
-  const float mult = row_factor<NORM, CODES>(p, row, sum, top, t == 0);
+  const RowFactor factor = row_factor<NORM, CODES>(p, row, sum, top, t == 0);
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
     const int c = first(n);
     if (c >= p.len) continue;
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[n][i] *= mult;
+    finish<NORM, CODES, V>(factor, v[n]);
     if (CODES) store_codes<V>(reinterpret_cast<uint8_t *>(packed) + (c + off), v[n]);
     else write(static_cast<T *>(p.y) + row * p.y_stride, c, v[n]);
   }
@@ -397,13 +430,14 @@ long_rows_kernel(const RowParams p) {
     if (CODES) top = max(top, __float_as_uint(times_gamma(v, c)) & 0x7fffffffu);
   }
   join<false>(sum, top, red);
-  const float mult = row_factor<NORM, CODES>(p, row, sum, top, threadIdx.x == 0);
+  const RowFactor factor = row_factor<NORM, CODES>(p, row, sum, top, threadIdx.x == 0);
   for (int c = threadIdx.x; c < p.len; c += blockDim.x) {
     const float v = value(c);
-    const float o = times_gamma(v, c) * mult;
+    float o[1] = {times_gamma(v, c)};
+    finish<NORM, CODES, 1>(factor, o);
     if (NORM && p.z) h[c] = from_f32<T>(v);
-    if (CODES) static_cast<uint8_t *>(p.y)[row * p.y_stride + c] = (uint8_t)e4m3x2(o, 0.f);
-    else static_cast<T *>(p.y)[row * p.y_stride + c] = from_f32<T>(o);
+    if (CODES) static_cast<uint8_t *>(p.y)[row * p.y_stride + c] = (uint8_t)e4m3x2(o[0], 0.f);
+    else static_cast<T *>(p.y)[row * p.y_stride + c] = from_f32<T>(o[0]);
   }
 }
 
