@@ -16,15 +16,22 @@ import torch
 from . import _lib
 from ._lib import ACTIVATIONS, TYPE_BF16, TYPE_E4M3, TYPE_F16, TYPE_F32, GemmScaledDesc, QuantizeDesc, RmsnormDesc, check
 
-try:
-    from . import torch_calls
-except ImportError as e:
-    raise ImportError("dace_onnx_b200/torch_calls.so is missing or does not fit this torch: build it with "
-                      "`python -m dace_onnx_b200.build` (%s)" % e) from e
+torch_calls = None  # the compiled module: opened by the first call, as libb200ops.so is
 
 FLOAT_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
 E4M3 = torch.float8_e4m3fn
 OPERAND_TYPES = {E4M3: TYPE_E4M3, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+
+
+def _calls():
+    global torch_calls
+    try:
+        from . import torch_calls as module
+    except ImportError as e:
+        raise ImportError("dace_onnx_b200/torch_calls.so is missing or does not fit this torch: build it with "
+                          "`python -m dace_onnx_b200.build` (%s)" % e) from e
+    torch_calls = module
+    return module
 
 
 def _act(activation):
@@ -138,7 +145,7 @@ def empty_codes(shape, device):
 
 
 def _rmsnorm(x, gamma, residual, eps, out, scale, residual_out, codes):
-    done = torch_calls.rmsnorm(x, gamma, residual, eps, out, scale, residual_out, codes)
+    done = (torch_calls or _calls()).rmsnorm(x, gamma, residual, eps, out, scale, residual_out, codes)
     if done is not None:
         if type(done) is int:
             check(done)
@@ -218,7 +225,7 @@ def quantize_rows(x, *, gate=None, activation=None, out=None, scale=None):
     activation: None / "none", "relu", "gelu", "gelu_tanh" or "silu"; it belongs to the gate. x and gate may be halves of one
     tensor (rows further apart than they are long)."""
     act = _act(activation)
-    done = torch_calls.quantize_rows(x, gate, act, out, scale)
+    done = (torch_calls or _calls()).quantize_rows(x, gate, act, out, scale)
     if done is not None:
         if type(done) is int:
             check(done)
@@ -289,8 +296,8 @@ def matmul_scaled(A, W, *, a_scale=None, w_scale=None, bias=None, activation=Non
     Operands whose rows do not start at multiples of 16 bytes are copied into such rows first: keep weights in a
     `PreparedLinear`, codes in tensors from `empty_codes` or the quantisers."""
     act = _act(activation)
-    done = torch_calls.matmul_scaled(A, W, a_scale, w_scale, bias, act, residual, out,
-                                     -1 if out_dtype is None else FLOAT_TYPES.get(out_dtype, TYPE_E4M3))
+    done = (torch_calls or _calls()).matmul_scaled(A, W, a_scale, w_scale, bias, act, residual, out,
+                                                   -1 if out_dtype is None else FLOAT_TYPES.get(out_dtype, TYPE_E4M3))
     if done is not None:
         if type(done) is int:
             check(done)
