@@ -193,13 +193,25 @@ PyObject *quantize_rows_impl(PyObject *const *a) {
   return r;
 }
 
-// A scale operand: one entry for all rows or one a row.
-bool scale_operand(PyObject *o, int device, int64_t rows, const float **p, int32_t *step) {
+// The axes that are not 1 agree with the first `axes` ones of `like`, or there is at most one (all rows in order).
+bool scale_shape(const at::Tensor &t, const at::Tensor &like, int64_t axes) {
+  int64_t i = 0, longer = 0;
+  bool agree = true;
+  for (int64_t j = 0; j < t.dim(); ++j) {
+    if (t.size(j) == 1) continue;
+    ++longer;
+    while (i < axes && like.size(i) == 1) ++i;
+    agree = agree && i < axes && like.size(i++) == t.size(j);
+  }
+  return agree || longer <= 1;
+}
+// A scale operand: one entry for all rows, or one for each row of `like` (whose rows lie along its first `axes` axes).
+bool scale_operand(PyObject *o, int device, const at::Tensor &like, int64_t axes, int64_t rows, const float **p, int32_t *step) {
   if (absent(o)) return true;
   const at::Tensor *t = tensor(o, device);
   if (!t || t->scalar_type() != at::kFloat || !t->is_contiguous()) return false;
   const int64_t n = t->numel();
-  if (n != rows && n != 1) return false;
+  if (n != 1 && (n != rows || !scale_shape(*t, like, axes))) return false;
   *step = n == rows;
   *p = static_cast<const float *>(t->data_ptr());
   return true;
@@ -228,7 +240,8 @@ PyObject *matmul_scaled_impl(PyObject *const *a) {
   d.ldw = row_stride(*W);
   if (!rows_for_tma(*A, d.lda, d.M, size) || !rows_for_tma(*W, d.ldw, d.N, size)) return not_ordinary();
   const float *a_scale = nullptr, *w_scale = nullptr;
-  if (!scale_operand(a[2], device, d.M, &a_scale, &d.a_scale_step) || !scale_operand(a[3], device, d.N, &w_scale, &d.w_scale_step))
+  if (!scale_operand(a[2], device, *A, A->dim() - 1, d.M, &a_scale, &d.a_scale_step) ||
+      !scale_operand(a[3], device, *W, 1, d.N, &w_scale, &d.w_scale_step))
     return not_ordinary();
   const at::Tensor *bias = nullptr, *residual = nullptr;
   if (!absent(a[4])) {

@@ -10,6 +10,7 @@ Ordinary calls go through `torch_calls`, which reads the tensors in C++; whateve
 are checked, errors raised and operands in other layouts copied.
 """
 import ctypes
+import math
 
 import torch
 
@@ -272,16 +273,22 @@ def _operand(t, size):
     return t, s
 
 
-def _scale_operand(t, name, rows, device):
+def _scale_shape(shape, lead):
+    """Whether a tensor of `shape` has one entry for each row of a tensor with leading axes `lead`, in their order: the axes that
+    are not 1 agree, or there is only one (all rows in order)."""
+    longer = [n for n in shape if n != 1]
+    return longer == [n for n in lead if n != 1] or (len(longer) <= 1 and math.prod(shape) == math.prod(lead))
+
+
+def _scale_operand(t, name, lead, device):
     """(tensor, step) of a scale operand: one entry for all rows, or one a row."""
     _on(device, t, name)
     if t.dtype is not torch.float32:
         raise TypeError("%s must be float32, got %s" % (name, t.dtype))
-    n = t.numel()
-    if n == rows:
+    if _scale_shape(t.shape, lead):
         return t if t.is_contiguous() else t.contiguous(), 1
-    if n != 1:
-        raise ValueError("%s must have one entry, or one for each of the %d rows" % (name, rows))
+    if t.numel() != 1:
+        raise ValueError("%s must have one entry, or one for each row: shape %s, got %s" % (name, tuple(lead), tuple(t.shape)))
     return t, 0
 
 
@@ -289,9 +296,9 @@ def matmul_scaled(A, W, *, a_scale=None, w_scale=None, bias=None, activation=Non
     """Y = activation((A W^T) * a_scale[:, None] * w_scale + bias) + residual, accumulated in fp32.
 
     A: [..., K], W: [N, K] (a Linear layer's layout), both e4m3 codes, float16 or bfloat16. a_scale: one fp32 entry a row of A
-    (A's leading shape) or one in all; w_scale: [N] or one in all. bias: [N], float32, float16 or bfloat16. activation: as in
-    `quantize_rows`. residual: the output's shape and type; it may be `out`. Output type: out's, or out_dtype, or the
-    residual's, or A's (bfloat16 for codes).
+    (A's leading shape, axes of 1 aside, or all rows along one axis) or one in all; w_scale: [N] or one in all. bias: [N],
+    float32, float16 or bfloat16. activation: as in `quantize_rows`. residual: the output's shape and type; it may be `out`.
+    Output type: out's, or out_dtype, or the residual's, or A's (bfloat16 for codes).
 
     Operands whose rows do not start at multiples of 16 bytes are copied into such rows first: keep weights in a
     `PreparedLinear`, codes in tensors from `empty_codes` or the quantisers."""
@@ -353,10 +360,10 @@ def matmul_scaled(A, W, *, a_scale=None, w_scale=None, bias=None, activation=Non
         bp = bias.data_ptr()
     sap, sa, swp, sw = None, 0, None, 0
     if a_scale is not None:
-        a_scale, sa = _scale_operand(a_scale, "a_scale", M, device)
+        a_scale, sa = _scale_operand(a_scale, "a_scale", shape[:-1], device)
         sap = a_scale.data_ptr()
     if w_scale is not None:
-        w_scale, sw = _scale_operand(w_scale, "w_scale", N, device)
+        w_scale, sw = _scale_operand(w_scale, "w_scale", (N,), device)
         swp = w_scale.data_ptr()
     size = 1 if code == TYPE_E4M3 else 2
     A, lda = _operand(A, size)
