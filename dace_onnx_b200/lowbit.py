@@ -388,6 +388,7 @@ class PreparedLinear:
         if dtype not in OPERAND_TYPES:
             raise TypeError("PreparedLinear: dtype must be float8_e4m3fn, float16 or bfloat16")
         _act(activation)
+        weight = weight.detach()  # the layer keeps values, not the graph of a parameter
         self.N, self.K = weight.shape
         self.activation, self.dtype = activation, dtype
         if bias is not None:
@@ -395,7 +396,7 @@ class PreparedLinear:
             _float_type(bias, "bias")
             if bias.shape != (self.N,):
                 raise ValueError("PreparedLinear: bias must be [%d]" % self.N)
-            bias = bias.contiguous()
+            bias = bias.detach().contiguous()
         self.bias = bias
         if dtype == E4M3:
             self.weight, self.w_scale = quantize_rows(weight)
