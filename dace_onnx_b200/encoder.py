@@ -94,13 +94,15 @@ class BertEncoderB200:
             h, f, nh = self.hidden, self.ffn, self.heads
             e = lambda *s: torch.empty(s, device=self.device, dtype=torch.float32)  # noqa: E731
             self._buf = dict(qkv=e(mb, seq, 3 * h), ctx=e(mb, seq, h), attn=e(mb, seq, h), h1=e(mb, seq, h),
-                             inter=e(mb, seq, f), out=e(mb, seq, h), ping=e(mb, seq, h), pong=e(mb, seq, h))
+                             out=e(mb, seq, h), ping=e(mb, seq, h), pong=e(mb, seq, h))
             if self.fp8:
                 self._buf.update(codes_h=ops.empty_codes((mb * seq, h), self.device),
                                  codes_f=ops.empty_codes((mb * seq, f), self.device), scale=e(mb * seq),
                                  # the Gelu's result, which is quantised next: its rounding to 8 bits of mantissa is a
                                  # sixteenth of e4m3's
                                  inter=torch.empty((mb, seq, f), device=self.device, dtype=torch.bfloat16))
+            else:
+                self._buf.update(inter=e(mb, seq, f))
             self._buf_key = key
         return self._buf
 
