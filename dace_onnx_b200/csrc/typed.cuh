@@ -130,13 +130,14 @@ __device__ __forceinline__ Pair over_one_plus_exp2(const Pair &x, const Pair &e)
 }
 __device__ __forceinline__ Pair both(float v) { return Pair(v, v); }
 
-// Activations of two fp32 values. All three smooth ones have the form x / (1 + 2^e(x)):
-//   silu       e = -log2(e) x
-//   gelu_tanh  0.5 (1 + tanh u) = 1 / (1 + exp(-2u)), so e = -2 log2(e) sqrt(2/pi) (x + 0.044715 x^3)
-//   gelu       Phi(x) = 1 / (1 + exp(-logit Phi(x))), and logit Phi(x) / x is an even, smooth function of x: a polynomial of
-//              degree 6 in x^2, fitted on |x| <= 6 by weighted least squares so that the error of x Phi(x) is at most 7.4e-8
-//              (and below 3e-4 of the value down to x = -4); past 6, where Phi is 0 or 1 to 1e-9, x^2 stays at 36.
-// Relative error otherwise that of an fp32 exponential, about (4 + |e|) 2^-24.
+// Activations of two fp32 values.
+//   silu       x / (1 + 2^e), e = -log2(e) x
+//   gelu_tanh  the same with 0.5 (1 + tanh u) = 1 / (1 + exp(-2u)): e = -2 log2(e) sqrt(2/pi) (x + 0.044715 x^3)
+//   gelu       x Phi(x) = max(x, 0) - |x| Phi(-|x|), and Phi(-w) = P(t) exp(-w^2 / 2) with t = 1 / (1 + 0.35 w): a polynomial without
+//              constant term of degree 9, fitted to erfcx(w / sqrt 2) / 2 on w <= 16 by reweighted least squares so that its relative
+//              error is at most 3.3e-8. The tail keeps its relative accuracy, which the scale of a row of negative gates needs.
+// Relative error: silu and gelu_tanh that of an fp32 exponential, about (4 + |e|) 2^-24; gelu below (16 + 1.25 x^2) 2^-24 for x < 0
+// and 4e-7 for x > 0 (2.4e-7 absolute anywhere). Values below 2^-126 come out as 0. NaN and gelu(-inf) give NaN.
 template <int ACT>
 __device__ __forceinline__ Pair activate2_t(const Pair &x) {
   if (ACT == B200_ACT_RELU) {
@@ -148,14 +149,26 @@ __device__ __forceinline__ Pair activate2_t(const Pair &x) {
   if (ACT == B200_ACT_GELU_TANH)
     return over_one_plus_exp2(x, x * fma2(x * x, both(-0.10294324f), both(-2.3022082f)));
   if (ACT == B200_ACT_GELU) {
-    float a, b;
-    (x * x).get(a, b);
-    const Pair q(fminf(a, 36.f), fminf(b, 36.f));
-    constexpr float c[7] = {-2.3022067f, -0.104839917f, 9.66251724e-05f, 0.000159056584f, -1.14027313e-05f, 3.81676884e-07f, -5.12706323e-09f};
-    Pair poly = both(c[6]);
+    float a, b, t0, t1, e0, e1;
+    x.get(a, b);
+    const Pair positive(fmaxf(a, 0.f), fmaxf(b, 0.f));
+    // +inf - 16 * 0, not inf * 0; -inf and NaN stay
+    asm("min.NaN.f32 %0, %0, 0f41800000;" : "+f"(a));
+    asm("min.NaN.f32 %0, %0, 0f41800000;" : "+f"(b));
+    const Pair w(fabsf(a), fabsf(b));
+    fma2(w, both(0.35f), both(1.f)).get(t0, t1);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(t0));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(t1));
+    (w * both(-0.7213475204444817f) * w).get(e0, e1);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e0));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e1));
+    constexpr float c[9] = {-0.139621243f, -0.139864519f, -0.119814187f, -0.105579816f, 0.0232753269f, -0.15940915f, 0.255915701f,
+                            -0.144067347f, 0.02916524f};  // of -P(t) / t
+    const Pair t(t0, t1);
+    Pair poly = both(c[8]);
 #pragma unroll
-    for (int i = 5; i >= 0; --i) poly = fma2(poly, q, both(c[i]));
-    return over_one_plus_exp2(x, x * poly);
+    for (int i = 7; i >= 0; --i) poly = fma2(poly, t, both(c[i]));
+    return fma2(w, poly * t * Pair(e0, e1), positive);
   }
   return x;
 }
