@@ -100,6 +100,7 @@ SIGNATURES = {
     "b200_transpose_2d_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64]),
     "b200_rmsnorm": (c_int, [c_void_p, POINTER(RmsnormDesc)] + [c_void_p] * 6),
     "b200_gemm_scaled": (c_int, [c_void_p, POINTER(GemmScaledDesc)] + [c_void_p] * 7),
+    "b200_gemm_scaled_plan": (c_int, [POINTER(GemmScaledDesc), c_void_p, c_void_p, POINTER(c_int32)]),
     "b200_quantize_rows": (c_int, [c_void_p, POINTER(QuantizeDesc)] + [c_void_p] * 4),
 }
 

@@ -19,13 +19,16 @@
 //          whose rows the pair kernel's vector accesses cannot address. Bound by memory and by its start and end: 32 x 28672,
 //          K 4096, e4m3 23 us (5.2 TB/s); one row, 4096 x 4096, 6 us.
 //
-// The tensor core adds into its fp32 accumulator with truncation, an error that grows with the number of additions. For
-// 16-bit outputs it stays far below their rounding; for fp32 outputs the sum is cut into chunks of kChunkKb K-blocks whose
-// accumulators the epilogue warps add in registers, rounding to nearest. The shorter the chunks, the sooner the issuing warp
-// runs out of accumulators while the epilogue stores (16384 x 4096 x 1024 to fp32, 16 and 32 additions: bf16 221K and 183K cycles,
-// e4m3 143K and 127K). Products of codes are short and lose little: with 32 additions the outputs are within 1.5e-7 of 64 bits
-// (2-norm, up to K = 16384, terms of one sign too). 16-bit operands lose more (32 additions: fp16 6.5e-7, terms of one sign
-// 2.5e-6) and keep 16.
+// The tensor core adds into its fp32 accumulator with truncation, an error that grows with the number of additions: up to 2^-24 of the
+// result for each when the terms have one sign. 16-bit outputs take all of K in one accumulator: 1792 additions for K = 28672 of
+// 16-bit operands, up to 1.1e-4 beside the output's own rounding of up to 4.9e-4 (fp16) or 3.9e-3 (bf16). For fp32 outputs the sum is
+// cut into chunks of kChunkKb K-blocks whose accumulators the epilogue warps add in registers, rounding to nearest. The shorter the
+// chunks, the sooner the issuing warp runs out of accumulators while the epilogue stores (16384 x 4096 x 1024 to fp32, 16 and 32
+// additions: bf16 221K and 183K cycles, e4m3 143K and 127K). Products of codes are short and lose little: with 32 additions the outputs
+// are within 1.0e-7 of 64 bits in the 2-norm up to K = 16384, 1.7e-7 with terms of one sign. 16-bit operands lose more (32 additions: fp16
+// 6.5e-7, terms of one sign 2.5e-6) and keep 16: fp16 3.6e-7 and 1.2e-6, bf16 2.5e-7 and 3.8e-7. The sums of 256 columns are 64 a thread,
+// more than its 112 registers hold beside the rest: the fp32 pair kernel spills (96 bytes stored, 528 loaded), part of its
+// distance to the 16-bit one (bf16 139K, e4m3 102K cycles).
 //
 // Every mbarrier wait is bounded by a cycle budget, as in gemm_tcgen05.cu.
 #include <cuda.h>
@@ -956,6 +959,12 @@ int row_access(const void *q, int64_t rows, int64_t ld, int bytes) {
   return bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : 0;
 }
 
+// The same for a call's outputs and residual together.
+int output_access(const b200_gemm_scaled_desc &d, const void *residual, const void *Y) {
+  const int vec = row_access(Y, d.M, d.ldy, type_bytes(d.y_type));
+  return residual ? min(vec, row_access(residual, d.M, d.ldr, type_bytes(d.y_type))) : vec;
+}
+
 bool is_float(int type) { return type == B200_TYPE_F32 || type == B200_TYPE_F16 || type == B200_TYPE_BF16; }
 
 }  // namespace
@@ -985,7 +994,7 @@ extern "C" B200_API int b200_gemm_scaled(void *stream, const b200_gemm_scaled_de
     return fail(B200_EINVAL, "gemm_scaled: leading dimension smaller than the row length");
   if (d.M > 0x7fffff00LL || d.N > 0x7fffff00LL || d.K > 0x7fffff00LL)
     return fail(B200_EUNSUPPORTED, "gemm_scaled: an extent is too large");
-  const int b = type_bytes(d.type), yb = type_bytes(d.y_type);
+  const int b = type_bytes(d.type);
   b200_gemm_scaled_desc e = d;
   // one row: its stride is never used, any valid one will do for the tensor map
   const int64_t pitch = (d.K * b + 15) / 16 * 16 / b;
@@ -994,7 +1003,19 @@ extern "C" B200_API int b200_gemm_scaled(void *stream, const b200_gemm_scaled_de
   if (!aligned16(A) || !aligned16(W) || e.lda * b % 16 || e.ldw * b % 16)
     return fail(B200_EUNSUPPORTED, "gemm_scaled: A and W need 16-byte aligned bases and row strides of multiples of 16 bytes");
   if (e.lda * b >= (1LL << 40) || e.ldw * b >= (1LL << 40)) return fail(B200_EUNSUPPORTED, "gemm_scaled: a row stride is too large");
-  int vec = row_access(Y, e.M, e.ldy, yb);
-  if (residual) vec = min(vec, row_access(residual, e.M, e.ldr, yb));
+  const int vec = output_access(e, residual, Y);
   return run_plan((cudaStream_t)stream, e, choose(e, vec >= 16), vec, A, W, a_scale, w_scale, bias, residual, Y);
+}
+
+extern "C" B200_API int b200_gemm_scaled_plan(const b200_gemm_scaled_desc *desc, const void *residual, const void *Y,
+                                              int32_t plan[3]) {
+  if (!desc || !plan) return fail(B200_EINVAL, "gemm_scaled_plan: null pointer");
+  if (desc->M < 1 || desc->N < 1 || desc->K < 1) return fail(B200_EINVAL, "gemm_scaled_plan: a product without outputs");
+  if ((desc->type != B200_TYPE_E4M3 && desc->type != B200_TYPE_F16 && desc->type != B200_TYPE_BF16) || !is_float(desc->y_type))
+    return fail(B200_EINVAL, "gemm_scaled_plan: unknown type");
+  const Plan p = choose(*desc, output_access(*desc, residual, Y) >= 16);
+  plan[0] = p.pair;
+  plan[1] = p.cols;
+  plan[2] = p.ranks;
+  return B200_OK;
 }

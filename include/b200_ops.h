@@ -320,6 +320,9 @@ typedef struct b200_gemm_scaled_desc {
 } b200_gemm_scaled_desc;
 B200_API int b200_gemm_scaled(void *stream, const b200_gemm_scaled_desc *desc, const void *A, const void *W,
                               const float *a_scale, const float *w_scale, const void *bias, const void *residual, void *Y);
+/* Which kernel such a call runs (nothing is launched or read): plan = {1, columns of a tile, 1} for the one of many rows, {0, rows of A
+ * a tile, CTAs over which K is split} for the one of few. */
+B200_API int b200_gemm_scaled_plan(const b200_gemm_scaled_desc *desc, const void *residual, const void *Y, int32_t plan[3]);
 
 #ifdef __cplusplus
 }
