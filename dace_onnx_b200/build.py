@@ -14,6 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB_PATH = os.path.join(HERE, "libb200ops.so")
 CALLS_PATH = os.path.join(HERE, "torch_calls.so")
+STAMP_PATH = os.path.join(HERE, "build", "torch_calls.stamp")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -25,8 +26,20 @@ def sources():
     return sorted(glob.glob(os.path.join(HERE, "csrc", "*.cu")))
 
 
+def _torch_stamp():
+    """What torch_calls.so is compiled against: the torch and the Python that load it must be these."""
+    from importlib import metadata
+    return "torch %s, python %d.%d" % (metadata.version("torch"), *sys.version_info[:2])
+
+
 def _stale():
     if not os.path.exists(LIB_PATH) or not os.path.exists(CALLS_PATH):
+        return True
+    try:
+        with open(STAMP_PATH) as f:
+            if f.read() != _torch_stamp():
+                return True
+    except FileNotFoundError:
         return True
     t = min(os.path.getmtime(LIB_PATH), os.path.getmtime(CALLS_PATH))
     deps = sources() + glob.glob(os.path.join(HERE, "csrc", "*.cpp")) + glob.glob(os.path.join(HERE, "csrc", "*.cuh")) + \
@@ -36,7 +49,7 @@ def _stale():
 
 def build(force=False, verbose=False):
     """Compile csrc/*.cu into libb200ops.so and csrc/torch_calls.cpp into torch_calls.so (skipped when both are newer than
-    their sources)."""
+    their sources and the torch is the one they were built for)."""
     if not force and not _stale():
         return LIB_PATH
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
@@ -65,6 +78,8 @@ def build(force=False, verbose=False):
     subprocess.check_call(
         ["g++", "-shared", "-o", CALLS_PATH, os.path.join(objdir, "torch_calls.o"), "-L" + torch_lib, "-lc10", "-lc10_cuda",
          "-ltorch_cpu", "-ltorch_python", "-L" + HERE, "-l:libb200ops.so", "-Wl,-rpath,$ORIGIN"])
+    with open(STAMP_PATH, "w") as f:
+        f.write(_torch_stamp())
     return LIB_PATH
 
 
