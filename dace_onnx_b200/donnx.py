@@ -96,7 +96,9 @@ def ONNXRMSNormalization(*, X, scale, Y, axis=-1, epsilon=1e-5, stash_type=1):
 def ONNXSkipSimplifiedLayerNormalization(*, input, skip, gamma, output, input_skip_bias_sum=None,  # noqa: A002
                                          epsilon=1e-5):
     """SkipSimplifiedLayerNormalization (com.microsoft, as exported for decoder models; not in the reference): RMS norm of
-    input + skip; input_skip_bias_sum, when passed, receives that sum."""
+    input + skip; input_skip_bias_sum, when passed, receives that sum. Without the node's optional bias, and with a skip of
+    the input's shape. epsilon: the node's attribute, which exporters write out; the default here is that of
+    RMSNormalization, not the schema's."""
     if input_skip_bias_sum is None:
         input_skip_bias_sum = torch.empty_like(input, memory_format=torch.contiguous_format)
 
