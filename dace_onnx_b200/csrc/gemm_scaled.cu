@@ -27,7 +27,7 @@
 // additions: bf16 221K and 183K cycles, e4m3 143K and 127K). Products of codes are short and lose little: with 32 additions the outputs
 // are within 1.0e-7 of 64 bits in the 2-norm up to K = 16384, 1.7e-7 with terms of one sign. 16-bit operands lose more (32 additions: fp16
 // 6.5e-7, terms of one sign 2.5e-6) and keep 16: fp16 3.6e-7 and 1.2e-6, bf16 2.5e-7 and 3.8e-7. The sums of 256 columns are 64 a thread,
-// more than its 112 registers hold beside the rest: the fp32 pair kernel spills (96 bytes stored, 528 loaded), part of its
+// more than its 96 registers hold beside the rest: the fp32 pair kernel spills (96 bytes stored, 528 loaded), part of its
 // distance to the 16-bit one (bf16 139K, e4m3 102K cycles).
 //
 // Every mbarrier wait is bounded by a cycle budget, as in gemm_tcgen05.cu.
@@ -172,6 +172,19 @@ __device__ __forceinline__ void finish_block(const ScaledParams &p, const float 
   }
 }
 
+template <typename OUT>
+__device__ __forceinline__ OUT ld_shared(uint32_t addr) {
+  if constexpr (sizeof(OUT) == 4) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+  } else {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+    return *reinterpret_cast<const OUT *>(&v);
+  }
+}
+
 // The loading and the issuing warp run converged, with one elected lane issuing: loop variables, addresses and
 // descriptors then live in uniform registers. (With a single lane in a branch of its own each of them had to be moved there for
 // every instruction: 170 clk per TMA load and 85 per MMA, against 128 clk that an MMA takes.)
@@ -250,7 +263,10 @@ __device__ __forceinline__ void tile_at(const ScaledParams &p, int64_t tile, int
   m_t = first + (int)(in - (int64_t)n_t * rows);
 }
 
-template <bool F8, typename OUT, int BN>
+// RAGGED: rows of Y end inside 16 bytes (they are further apart than they are long). A TMA store is cut off at the tensor's edge in
+// pieces of 16 bytes, so it would write behind such an end: there each thread stores the last block of its row itself, value
+// by value. (A variant of its own: with the branch in every instance 16384 x 4096 x 1024 e4m3 took 76 us, without 68.)
+template <bool F8, typename OUT, int BN, bool RAGGED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN, OUT>::kThreads, 1)
 scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                    const __grid_constant__ CUtensorMap map_y, const ScaledParams p) {
@@ -412,6 +428,19 @@ scaled_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         __syncwarp();
         if (p.residual) finish_block<OUT, true>(p, v, sa, sw + c, bs + c, r ? r + c : nullptr, cols, my_row, flip);
         else finish_block<OUT, false>(p, v, sa, sw + c, bs + c, nullptr, cols, my_row, flip);
+        if (RAGGED && cols < B) {  // uniform
+          if (m0 + lane < p.M) {
+            OUT *y = static_cast<OUT *>(p.Y) + (m0 + lane) * p.ldy + n0 + c;
+#pragma unroll 1
+            for (int i = 0; i < cols; ++i) {
+              const uint32_t piece = (uint32_t)i * sizeof(OUT) / 16, in = (uint32_t)i * sizeof(OUT) % 16;
+              y[i] = ld_shared<OUT>(my_row + ((piece ^ flip) << 4) + in);
+            }
+          }
+          if (lane == 0) bulk_commit();  // an empty group: the wait above counts one for each block
+          __syncwarp();
+          return;
+        }
         fence_async_shared();
         __syncwarp();
         if (lane == 0) {
@@ -807,10 +836,10 @@ struct Operands {
   int type, y_type;
 };
 
-template <bool F8, typename OUT, int BN>
+template <bool F8, typename OUT, int BN, bool RAGGED>
 int launch_pair(cudaStream_t st, const Operands &o, ScaledParams &p) {
   using C = PairCfg<BN, OUT>;
-  auto kern = scaled_pair_kernel<F8, OUT, BN>;
+  auto kern = scaled_pair_kernel<F8, OUT, BN, RAGGED>;
   static std::atomic<uint64_t> smem_set{0};
   if (int rc = raise_smem(kern, C::kSmemBytes, smem_set)) return rc;
   // the clusters the device holds at once: a persistent grid must not exceed them (per device, never changes)
@@ -868,7 +897,11 @@ int launch_split(cudaStream_t st, const Operands &o, ScaledParams &p, int ranks)
 
 template <bool F8, typename OUT>
 int launch_plan(cudaStream_t st, const Operands &o, ScaledParams &p, const Plan &plan) {
-  if (plan.pair) return plan.cols == 256 ? launch_pair<F8, OUT, 256>(st, o, p) : launch_pair<F8, OUT, 128>(st, o, p);
+  if (plan.pair) {
+    if (p.N * (int64_t)sizeof(OUT) % 16 == 0)
+      return plan.cols == 256 ? launch_pair<F8, OUT, 256, false>(st, o, p) : launch_pair<F8, OUT, 128, false>(st, o, p);
+    return plan.cols == 256 ? launch_pair<F8, OUT, 256, true>(st, o, p) : launch_pair<F8, OUT, 128, true>(st, o, p);
+  }
   switch (plan.cols) {
     case 16: return launch_split<F8, OUT, 16>(st, o, p, plan.ranks);
     case 32: return launch_split<F8, OUT, 32>(st, o, p, plan.ranks);
