@@ -78,3 +78,13 @@ def test_small_rows_and_small_eps(length, cuda):
     y = x * 2.0 ** 30
     same(ops.rmsnorm_quantize(x, eps=eps), expected(y))
     assert torch.equal(ops.rmsnorm(x, eps=eps), y)
+
+
+@pytest.mark.parametrize("length", [64, 333, 4096, 40000])
+def test_rows_of_any_magnitude(length, cuda):
+    """A power of two moves to the scale: the codes stay, from values near the floor of a row's maximum to values near overflow."""
+    x = make(9, 5, length).clamp(-7.9, 7.9)
+    x[:, 0] = 2.0
+    q, s = ops.quantize_rows(x)
+    for k in (-99, -60, 60, 100, 125):
+        same(ops.quantize_rows(x * 2.0 ** k), (q, s * 2.0 ** k))
