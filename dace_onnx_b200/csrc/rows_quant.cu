@@ -134,13 +134,24 @@ __device__ __forceinline__ void gate_vec(float (&v)[VEC], const float (&z)[VEC])
   }
 }
 
+// The largest |v|, or NaN: one instruction for two values.
+template <int VEC>
+__device__ __forceinline__ void largest(float &top, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(v[0])));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(fabsf(v[i])), "f"(fabsf(v[i + 1])));
+  }
+}
+
 __device__ __forceinline__ uint32_t warp_umax(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
 // Sum and maximum over the threads of a row. WARP: a warp is a row. Otherwise the CTA is; `red` holds 2 x 32 words.
 template <bool WARP>
-__device__ __forceinline__ void join(float &sum, uint32_t &top, float *red) {
+__device__ __forceinline__ void join(float &sum, float &largest, float *red) {
   sum = warp_sum(sum);
-  top = warp_umax(top);
+  uint32_t top = warp_umax(__float_as_uint(largest));
   if (!WARP) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
     if (lane == 0) {
@@ -152,6 +163,7 @@ __device__ __forceinline__ void join(float &sum, uint32_t &top, float *red) {
     sum = warp_sum(lane < nwarp ? red[lane] : 0.f);
     top = warp_umax(lane < nwarp ? __float_as_uint(red[32 + lane]) : 0u);
   }
+  largest = __uint_as_float(top);
 }
 
 // `top` is the pattern of max|y|: the floor keeps 448 / max finite; a NaN fails the comparison and stays.
@@ -186,10 +198,10 @@ struct RowFactor {
 };
 // From the row's sum of squares and largest pattern; the first thread of the row stores its scale.
 template <bool NORM, bool CODES>
-__device__ __forceinline__ RowFactor row_factor(const RowParams &p, int64_t row, float sum, uint32_t top, bool first) {
+__device__ __forceinline__ RowFactor row_factor(const RowParams &p, int64_t row, float sum, float top, bool first) {
   const float rho = NORM ? 1.f / sqrtf(sum / (float)p.len + p.eps) : 1.f;
   if (!CODES) return RowFactor{rho, 1.f, 0.f};
-  const float scale = row_max(__uint_as_float(top) * rho) / kE4M3Max;
+  const float scale = row_max(top * rho) / kE4M3Max;
   if (first) p.scale[row] = scale;
   // an infinite scale makes quotients of finite values 0, which need no correction (and 0 * inf would be none)
   return RowFactor{rho, 1.f / scale, scale == INFINITY ? 0.f : -scale};
@@ -252,7 +264,7 @@ rows_kernel(const RowParams p) {
   }
   float v[NV][VEC];
   float sum = 0.f;
-  uint32_t top = 0;
+  float top = 0.f;
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
     const int c = (n * lanes + t) * VEC;
@@ -274,10 +286,7 @@ rows_kernel(const RowParams p) {
         for (int i = 0; i < VEC; ++i) v[n][i] *= g[i];
       }
     }
-    if (CODES) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(v[n][i]) & 0x7fffffffu);
-    }
+    if (CODES) largest<VEC>(top, v[n]);
   }
   join<WARP>(sum, top, red);
   const RowFactor factor = row_factor<NORM, CODES>(p, row, sum, top, t == 0);
@@ -336,7 +345,7 @@ shifted_rows_kernel(const RowParams p) {
   }
   float v[NV][V];
   float sum = 0.f;
-  uint32_t top = 0;
+  float top = 0.f;
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
     const int c = first(n);
@@ -363,10 +372,7 @@ shifted_rows_kernel(const RowParams p) {
         }
       }
     }
-    if (CODES) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(v[n][i]) & 0x7fffffffu);
-    }
+    if (CODES) largest<V>(top, v[n]);
   }
   join<false>(sum, top, red);
   const RowFactor factor = row_factor<NORM, CODES>(p, row, sum, top, t == 0);
@@ -423,11 +429,12 @@ long_rows_kernel(const RowParams p) {
     return v * (p.gamma_f32 ? static_cast<const float *>(p.gamma)[c] : to_f32<T>(static_cast<const T *>(p.gamma)[c]));
   };
   float sum = 0.f;
-  uint32_t top = 0;
+  float top = 0.f;
   for (int c = threadIdx.x; c < p.len; c += blockDim.x) {
     const float v = value(c);
     if (NORM) sum = fmaf(v, v, sum);
-    if (CODES) top = max(top, __float_as_uint(times_gamma(v, c)) & 0x7fffffffu);
+    const float g[1] = {times_gamma(v, c)};
+    if (CODES) largest<1>(top, g);
   }
   join<false>(sum, top, red);
   const RowFactor factor = row_factor<NORM, CODES>(p, row, sum, top, threadIdx.x == 0);
