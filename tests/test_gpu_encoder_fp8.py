@@ -70,3 +70,22 @@ def test_every_step_of_a_layer(hidden, heads, ffn, shape, cuda):
     linear(b["inter"], b["h1"], p["wi"], p["bi"], act="gelu")
     linear(b["out"], b["inter"], p["wo2"], p["bo2"], residual=b["h1"])
     norm(y, b["out"], p["ln2_g"], p["ln2_b"])
+
+
+def test_two_encoders_at_once(cuda):
+    """Products, attention and norms of two models on two streams, TMEM and shared memory shared as the kernels meet: the same bits as
+    one after the other."""
+    encs = [BertEncoderB200([po.make_bert_layer_params(256, 1024, seed=s)] * 2, heads=4, device=cuda, math_mode=mode)
+            for s, mode in ((8, "fp8"), (9, "fp8"), (10, "tf32"))]
+    xs = [torch.randn(n, 128, 256, generator=torch.Generator().manual_seed(n)).to(cuda) for n in (2, 24, 12)]
+    want = [e.forward_device(x).clone() for e, x in zip(encs, xs)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in encs]
+    got = [[] for _ in encs]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(encs[i].forward_device(xs[i]))
+    torch.cuda.synchronize()
+    for w, ys in zip(want, got):
+        assert all(torch.equal(w, y) for y in ys)
