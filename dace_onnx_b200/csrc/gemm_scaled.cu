@@ -10,7 +10,7 @@
 //   pair   many rows of A. A cluster of two CTAs computes 256 x BN outputs (rows of A are TMEM lanes), persistent, several
 //          accumulators so that the epilogue of a tile runs under the MMAs of the next. Outputs leave through shared memory and
 //          TMA stores: 32-byte stores of each thread's own row took a third of the epilogue. Bound by the power limit: 8192 x
-//          14336, K 4096, e4m3 with bias and silu 384 us (2.5 PFLOP/s) at 1000 W and 1.1 to 1.2 GHz.
+//          14336, K 4096, e4m3 with bias and silu 387 to 406 us (2.4 to 2.5 PFLOP/s) at 1000 W and 1.1 to 1.2 GHz.
 //   split  few rows of A, where the weights' bytes bound the product and there are fewer tiles than SMs. Operands
 //          change places: 128 rows of W are the TMEM lanes and NT rows of A the columns, so that a single token fills
 //          the tensor core's wide side with weights. K is split over the CTAs of a cluster (at most 8), whose partial

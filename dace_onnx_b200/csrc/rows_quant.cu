@@ -7,12 +7,12 @@
 // Both are bound by memory: each input is read once, each output written once. A row stays in the registers of the
 // threads that loaded it (up to 32 values a thread). The norm needs two reductions over the row, sum(h^2) and max|y|;
 // because rho is a positive factor common to the row, max|y| = rho * max|h * gamma|, so both are taken in ONE pass
-// over the registers and joined in one exchange between warps. The maximum runs on the bit patterns of |y| as
-// unsigned integers: they order like the values, and a NaN's pattern is above infinity's, so a NaN reaches the scale.
+// over the registers and joined in one exchange between warps. The maximum keeps a NaN, so that it reaches the scale; between threads it
+// runs on bit patterns as unsigned integers, which order like the values, with a NaN's above infinity's.
 //
-// Measured over three sets of data in rotation (bytes read and written once / time): 8192 x 8192 bf16 norm with residual to e4m3 76
-// us, 6.2 TB/s; 16384 x 1024 fp32 the same 36 us, 6.0 TB/s; 8192 x 14336 bf16 silu(gate) * x 103 us, 5.7 TB/s; 16384 x 4096 fp32
-// 57 us, 5.9 TB/s. A copy runs at 6.5 TB/s.
+// Measured over three sets of data in rotation, sustained (bytes read and written once / time; boards differ by up to 6 %): 8192 x 8192 bf16
+// norm with residual to e4m3 81 us, 5.8 TB/s; 16384 x 1024 fp32 the same 36 us, 6.1 TB/s; 8192 x 14336 bf16 silu(gate) * x 105 us, 5.6
+// TB/s; 16384 x 4096 fp32 59 us, 5.7 TB/s. A copy runs at 6.5 TB/s.
 #include <math.h>
 
 #include "typed.cuh"
@@ -484,7 +484,7 @@ int dispatch(cudaStream_t st, const RowParams &p, Rows rows) {
   const int per = vec ? V : 1;                     // values of one access
   const int units = (p.len + per - 1) / per;       // accesses of a row (len is a multiple of V when vec)
   // Many rows: about one CTA starts per nanosecond, so short rows are put eight to a CTA, a warp each (131072 x 256 bf16 norm
-  // 42 us, a CTA each 70; 60000 x 333 value by value 60 and 69). A longer row is a CTA's: two accesses a thread, four where
+  // 42 us, a CTA each 70; 60000 x 333 value by value 60 and 69; these and the times below before codes were quotients). A longer row is a CTA's: two accesses a thread, four where
   // one 16-bit input leaves few bytes on the way (8192 x 8192 bf16 quantise 48 -> 36 us, norm 73 either way), and more until the
   // CTA has at most 512 threads (norm with 1024 threads 84 us), but for the spills of eight (8192 x 14336 fp32 norm 272 us, 896
   // threads with four 235). Few rows leave SMs idle: one access each, the shortest way through a row.
